@@ -103,6 +103,17 @@ SIGNATURES = {
     "ea_silu_f32": (_i, [_vp, _vp, _ll, _vp]),
     "ea_add_f16": (_i, [_vp, _vp, _vp, _ll, _vp]),
     "ea_lincomb_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp]),
+    "ea_quantize_fp8": (_i, [_vp, _i, _vp, _vp, _ll, _i, _vp]),
+    "ea_quantize_fp8_weight": (_i, [_vp, _i, _vp, _vp, _i, _i, _vp]),
+    "ea_dequantize_fp8": (_i, [_vp, _vp, _i, _vp, _i, _ll, _i, _vp]),
+    "ea_activation_fp8": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _i, _vp]),
+    "ea_activation_fp8_bwd": (_i, [_vp, _vp, _vp, _i, _vp, _ll, _i, _vp]),
+    "ea_layernorm_train": (_i, [_vp, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "ea_layernorm_bwd_workspace_bytes": (_sz, [_i, _i]),
+    "ea_layernorm_bwd": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp, _sz, _vp]),
+    "ea_gemm_fp8": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, C.POINTER(Epilogue), _vp]),
+    "ea_gemm_fp8_wgrad_workspace_bytes": (_sz, [_i, _i, _i]),
+    "ea_gemm_fp8_wgrad": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
     "ea_gather_rows": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp]),
 }
 

@@ -1,0 +1,119 @@
+// ea_fp8.h -- the 8-bit block format shared by ea_train.hip, ea_fp8.hip and ea_fp8_gemm.hip.
+//
+// A row of C values is cut into blocks of 128 (the last one padded with zero codes).  A block holds e4m3 codes (OCP: 4 exponent
+// bits, 3 mantissa bits, largest 448, no infinity) and ONE exponent E: a code stands for code * 2^E.
+//   E = the smallest whole number with max |x| <= 448 * 2^E  over the block's finite values (0 for a block of zeros), in
+//   [-100, 120]; stored as the byte E + 127 (E8M0), which is what the matrix instruction v_mfma_scale_f32_16x16x128_f8f6f4 takes.
+// A power of two costs a floating format nothing but the unused part of its top octave, makes x * 2^-E exact (the code is the only
+// rounding: at most 2^-4 of the value, or 2^-10 * 2^E), and lets the matrix unit apply both operands' scales inside the product.
+// Non-finite values become NaN codes (e4m3 has no infinity) and do not enter the maximum.
+//   codes   [rows][Kp], Kp = C rounded up to 128
+//   scales  [Kp / 128][Rp], Rp = rows rounded up to 16 (block-major: four consecutive rows' bytes are one 32-bit load)
+//           a weight shares one exponent among 128 rows: [Kp / 128][ceil(rows / 128)]
+#pragma once
+#include "ea_platform.h"
+#include "ea_prims.h"
+
+#define EA_FP8_BLOCK 128
+#define EA_FP8_E_MIN (-100)
+#define EA_FP8_E_MAX 120
+
+__device__ __forceinline__ unsigned ea_f2u(float v) { return __builtin_bit_cast(unsigned, v); }
+__device__ __forceinline__ float ea_u2f(unsigned v) { return __builtin_bit_cast(float, v); }
+// |v| where it enters a block's maximum: NaN and infinity count as 0
+__device__ __forceinline__ float ea_finite_abs(float v) {
+  const unsigned u = ea_f2u(v) & 0x7fffffffu;
+  return u < 0x7f800000u ? ea_u2f(u) : 0.0f;
+}
+// the block's exponent byte from its maximum: 448 = 1.75 * 2^8
+__device__ __forceinline__ int ea_fp8_exp_byte(float amax) {
+  const unsigned u = ea_f2u(amax);
+  int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = e < EA_FP8_E_MIN ? EA_FP8_E_MIN : (e > EA_FP8_E_MAX ? EA_FP8_E_MAX : e);
+  return (u == 0 ? 0 : e) + 127;
+}
+__device__ __forceinline__ float ea_fp8_scale(int byte) { return ea_u2f((unsigned)byte << 23); }            // 2^E
+__device__ __forceinline__ float ea_fp8_inv_scale(int byte) { return ea_u2f((unsigned)(254 - byte) << 23); }  // 2^-E
+
+#ifdef EA_EMU
+inline float ea_emu_fp8_to_f32(unsigned c) {
+  const int s = c >> 7, e = (c >> 3) & 15, m = c & 7;
+  if (e == 15 && m == 7) return NAN;
+  const float v = e ? ldexpf(1.0f + m / 8.0f, e - 7) : ldexpf((float)m, -9);
+  return s ? -v : v;
+}
+inline unsigned ea_emu_f32_to_fp8(float x) {   // round to nearest even; the callers keep |x| <= 448
+  if (x != x) return 0x7f;
+  const unsigned s = signbit(x) ? 0x80 : 0;
+  const float a = fabsf(x);
+  int e;
+  frexpf(a < 0.015625f ? 0.015625f : a, &e);
+  const float step = ldexpf(1.0f, e - 4);
+  const float r = nearbyintf(a / step) * step;
+  if (r >= 0.015625f) {
+    int e2;
+    const float f = frexpf(r, &e2);
+    return s | (unsigned)((e2 - 1 + 7) << 3) | (unsigned)((f * 2.0f - 1.0f) * 8.0f);
+  }
+  return s | (unsigned)(r * 512.0f);
+}
+__device__ __forceinline__ unsigned ea_fp8_pack4(float a, float b, float c, float d) {
+  return ea_emu_f32_to_fp8(a) | ea_emu_f32_to_fp8(b) << 8 | ea_emu_f32_to_fp8(c) << 16 | ea_emu_f32_to_fp8(d) << 24;
+}
+__device__ __forceinline__ void ea_fp8_unpack4(unsigned w, float* v) {
+  for (int i = 0; i < 4; ++i) v[i] = ea_emu_fp8_to_f32((w >> (8 * i)) & 255);
+}
+#else
+__device__ __forceinline__ unsigned ea_fp8_pack4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+__device__ __forceinline__ void ea_fp8_unpack4(unsigned w, float* v) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
+}
+#endif
+// x * 2^-E ready for the conversion: what is not finite becomes a NaN code
+__device__ __forceinline__ float ea_fp8_prep(float x, float inv) {
+  return (ea_f2u(x) & 0x7fffffffu) < 0x7f800000u ? x * inv : ea_u2f(0x7fc00000u);
+}
+// 8 values -> 8 codes
+__device__ __forceinline__ u32x2 ea_fp8_encode8(const float* v, float inv) {
+  float t[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = ea_fp8_prep(v[j], inv);
+  return u32x2{ea_fp8_pack4(t[0], t[1], t[2], t[3]), ea_fp8_pack4(t[4], t[5], t[6], t[7])};
+}
+
+// ---- reductions over aligned groups of LPR lanes (8, 16, 32, 64); every lane gets the result.  Up to 16 lanes they stay in the
+// vector unit (DPP: quad permutes, half-row mirror, row rotate); 32 and 64 add a lane exchange.
+#ifdef EA_EMU
+#define EA_DPP(v, ctrl, mask) ea_shfl_xor(v, mask)
+#else
+template <int CTRL>
+__device__ __forceinline__ float ea_dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+#define EA_DPP(v, ctrl, mask) ea_dpp<ctrl>(v)
+#endif
+template <int LPR, typename F>
+__device__ __forceinline__ float ea_group_reduce(float v, F f) {
+  v = f(v, EA_DPP(v, 0xB1, 1));                 // quad_perm [1, 0, 3, 2]
+  v = f(v, EA_DPP(v, 0x4E, 2));                 // quad_perm [2, 3, 0, 1]
+  v = f(v, EA_DPP(v, 0x141, 4));                // row_half_mirror: the other quad of the 8 (all four lanes of a quad agree)
+  if (LPR >= 16) v = f(v, EA_DPP(v, 0x128, 8)); // row_ror:8
+  if (LPR >= 32) v = f(v, ea_shfl_xor(v, 16));
+  if (LPR >= 64) v = f(v, ea_shfl_xor(v, 32));
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ float ea_group_sum(float v) {
+  return ea_group_reduce<LPR>(v, [](float a, float b) { return a + b; });
+}
+template <int LPR>
+__device__ __forceinline__ float ea_group_max(float v) {
+  return ea_group_reduce<LPR>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
+static inline int ea_fp8_blocks(int cols) { return (cols + EA_FP8_BLOCK - 1) / EA_FP8_BLOCK; }
+static inline long long ea_fp8_scale_pitch(long long rows) { return (rows + 15) / 16 * 16; }

@@ -1,0 +1,356 @@
+// ea_fp8.hip -- activations and weights in 8 bits (format: ea_fp8.h): quantisation of rows and of 128 x 128 weight blocks, its
+// inverse, and activation functions that keep their INPUT in 8 bits for the backward pass.
+//
+//   save   h = f(z),  saved = q8(z)         f: SiLU, exact GELU, GEGLU (h = value * gelu(gate), z = [value | gate]); h fp16 or q8(h)
+//   use    dz = dh f'(z),  z decoded from `saved`
+//             SiLU'(z) = s (1 + z (1 - s)), s = sigmoid(z);   GELU'(z) = Phi(z) + z phi(z)
+// Each is one pass bound by HBM.  Sixteen lanes own one block of 128 (a 16-byte load of 8 values each), so the block's maximum is
+// four DPP steps and the codes go out as 128 contiguous bytes; a workgroup covers 16 rows x 4 blocks, four blocks' loads in flight per
+// lane, and the 16 rows' scale bytes of a block are adjacent.
+#include "ea_fp8.h"
+#include "../../include/editanything_hip.h"
+
+namespace {
+
+constexpr int Q_KB = 4;        // blocks of 128 columns per thread
+
+template <bool F32, bool VEC>
+__device__ __forceinline__ void q_load8(const void* x, long long row, int cols, int c, float* v) {
+  if constexpr (VEC) {
+    const int cc = c < cols ? c : 0;                          // clamped, unconditional loads: four blocks in flight
+    if constexpr (F32) {
+      const float* p = (const float*)x + row * cols + cc;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    } else {
+      const f16x8 h = ea_ld8((const f16*)x + row * cols + cc);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+    }
+    if (c >= cols)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = c + j < cols ? (F32 ? ((const float*)x)[row * cols + c + j] : (float)((const f16*)x)[row * cols + c + j]) : 0.0f;
+  }
+}
+
+__device__ __forceinline__ void q_store(const float* v, uint8_t* q, uint8_t* scale, long long row, int Kp, long long Rp, int kb, int l,
+                                        bool live) {        // every lane of the wave calls it; rows that are not there store nothing
+  float m = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = fmaxf(m, ea_finite_abs(v[j]));
+  const int e = ea_fp8_exp_byte(ea_group_max<16>(m));
+  const u32x2 w = ea_fp8_encode8(v, ea_fp8_inv_scale(e));
+  if (live) *reinterpret_cast<u32x2*>(q + row * Kp + kb * 128 + l * 8) = w;
+  if (live && l == 0) scale[(long long)kb * Rp + row] = (uint8_t)e;
+}
+
+// ----------------------------------------------------------------------------------------------------- rows -> 8 bits
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(256) void ea_quant_rows_kernel(const void* x, uint8_t* q, uint8_t* scale, long long rows, int cols, int nb,
+                                                            long long Rp, int gx) {
+  const int l = threadIdx.x & 15;
+  const long long rt = blockIdx.x / gx;
+  const long long row = rt * 16 + (threadIdx.x >> 4);
+  const int kb0 = (blockIdx.x - (int)(rt * gx)) * Q_KB;
+  const bool live = row < rows;
+  const long long r = live ? row : rows - 1;
+  float v[Q_KB][8];
+#pragma unroll
+  for (int u = 0; u < Q_KB; ++u) q_load8<F32, VEC>(x, r, cols, (kb0 + u) * 128 + l * 8, v[u]);
+#pragma unroll
+  for (int u = 0; u < Q_KB; ++u)
+    if (kb0 + u < nb) q_store(v[u], q, scale, row, nb * 128, Rp, kb0 + u, l, live);
+}
+
+// ------------------------------------------------------------------------------------------- a 128 x 128 weight block
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(256) void ea_quant_weight_kernel(const void* w, uint8_t* q, uint8_t* scale, int N, int K, int nb) {
+  EA_SMEM(smem);
+  float* red = reinterpret_cast<float*>(smem);
+  const int l = threadIdx.x & 15, gy = threadIdx.x >> 4, kb = blockIdx.x;
+  const int n0 = blockIdx.y * 128;
+  float v[8][8];
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = n0 + gy + 16 * i;
+    q_load8<F32, VEC>(w, n < N ? n : N - 1, K, kb * 128 + l * 8, v[i]);      // (a repeated last row leaves the maximum as it is)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, ea_finite_abs(v[i][j]));
+  }
+  m = ea_group_max<64>(m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  const int e = ea_fp8_exp_byte(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+  const float inv = ea_fp8_inv_scale(e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = n0 + gy + 16 * i;
+    if (n < N) *reinterpret_cast<u32x2*>(q + (long long)n * nb * 128 + kb * 128 + l * 8) = ea_fp8_encode8(v[i], inv);
+  }
+  if (threadIdx.x == 0) scale[(long long)kb * gridDim.y + blockIdx.y] = (uint8_t)e;
+}
+
+// ------------------------------------------------------------------------------------------------------ 8 bits -> rows
+__device__ __forceinline__ void q_decode8(const uint8_t* p, float s, float* v) {
+  const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+  ea_fp8_unpack4(w[0], v);
+  ea_fp8_unpack4(w[1], v + 4);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= s;
+}
+template <bool VEC>
+__device__ __forceinline__ void h_load8(const f16* p, int c, int cols, float* v) {
+  if constexpr (VEC) {
+    const f16x8 h = ea_ld8(p + (c < cols ? c : 0));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? (float)p[c + j] : 0.0f;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void h_store8(f16* p, int c, int cols, const float* v) {
+  if constexpr (VEC) {
+    f16x8 h;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = (f16)v[j];
+    if (c < cols) ea_st8(p + c, h);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) p[c + j] = (f16)v[j];
+  }
+}
+
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(256) void ea_dequant_kernel(const uint8_t* q, const uint8_t* scale, void* out, long long rows, int cols, int nb,
+                                                         long long pitch, int row_shift, int gx) {
+  const int l = threadIdx.x & 15;
+  const long long rt = blockIdx.x / gx;
+  const long long row = rt * 16 + (threadIdx.x >> 4);
+  const int kb0 = (blockIdx.x - (int)(rt * gx)) * Q_KB;
+  if (row >= rows) return;
+#pragma unroll
+  for (int u = 0; u < Q_KB; ++u) {
+    const int kb = kb0 + u, c = kb * 128 + l * 8;
+    if (kb >= nb) break;
+    float v[8];
+    q_decode8(q + row * nb * 128 + c, ea_fp8_scale(scale[kb * pitch + (row >> row_shift)]), v);
+    if constexpr (F32) {
+      float* o = (float*)out + row * cols;
+      if (VEC && c < cols) {
+        *reinterpret_cast<f32x4*>(o + c) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(o + c + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      } else if (!VEC) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j < cols) o[c + j] = v[j];
+      }
+    } else h_store8<VEC>((f16*)out + row * cols, c, cols, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ activation, forward
+struct ActParams {
+  const f16* z; f16* h; uint8_t* hq; uint8_t* hs;      // forward: z [M][g H], h fp16 or 8-bit
+  uint8_t* zq; uint8_t* zs;                            // z as [g M][H] rows in 8 bits
+  const f16* dh; f16* dz;                              // backward
+  long long M; int H, nb, gx; long long RpH, RpZ;
+};
+
+template <int ACT>
+__device__ __forceinline__ float act_f(float z) { return ACT == EA_ACT_SILU ? ea_silu(z) : ea_gelu_erf(z); }
+
+// Phi(x) and x phi(x); 1 - Phi(a) = erfc(a / sqrt 2) / 2 as in ea_gelu_erf
+__device__ __forceinline__ void gelu_parts(float x, float& phi_c, float& xp) {
+  const float a = fminf(fabsf(x), 5.65685424949238f);
+  float q = -4.276626896171365e-06f;
+  q = q * a + 1.2775987670465838e-05f;
+  q = q * a + 0.0005758762708865106f;
+  q = q * a - 0.007670961786061525f;
+  q = q * a + 0.05294874310493469f;
+  q = q * a + 0.45904383063316345f;
+  q = q * a + 1.1511269807815552f;
+  const float t = ea_exp2_raw(-a * q - 1.0f);
+  phi_c = x > 0.0f ? 1.0f - t : t;
+  xp = x * 0.3989422804014327f * ea_exp2_raw(fmaxf(x * x * -0.7213475204444817f, -126.0f));
+  if (x != x) phi_c = xp = x;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if (ACT == EA_ACT_SILU) {
+    const float s = 1.0f / (1.0f + ea_expf(-z));
+    return s * (1.0f + z * (1.0f - s));
+  }
+  float P, xp;
+  gelu_parts(z, P, xp);
+  return P + xp;
+}
+
+template <int ACT, bool VEC, bool OUT8>
+__global__ __launch_bounds__(256) void ea_act_save_kernel(ActParams p) {
+  constexpr int G = ACT == EA_ACT_GEGLU ? 2 : 1;
+  const int l = threadIdx.x & 15;
+  const long long rt = blockIdx.x / p.gx;
+  const long long row = rt * 16 + (threadIdx.x >> 4);
+  const int kb0 = (blockIdx.x - (int)(rt * p.gx)) * Q_KB;
+  const bool live = row < p.M;
+  const long long r = live ? row : p.M - 1;
+  float v[G][Q_KB][8];
+#pragma unroll
+  for (int u = 0; u < Q_KB; ++u)
+#pragma unroll
+    for (int g = 0; g < G; ++g) q_load8<false, VEC>(p.z, r * G + g, p.H, (kb0 + u) * 128 + l * 8, v[g][u]);
+#pragma unroll
+  for (int u = 0; u < Q_KB; ++u) {
+    const int kb = kb0 + u, c = kb * 128 + l * 8;
+    if (kb >= p.nb) break;
+#pragma unroll
+    for (int g = 0; g < G; ++g) q_store(v[g][u], p.zq, p.zs, row * G + g, p.nb * 128, p.RpZ, kb, l, live);
+    float h[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = G == 2 ? v[0][u][j] * act_f<EA_ACT_GELU>(v[G - 1][u][j]) : act_f<ACT>(v[0][u][j]);
+    if constexpr (OUT8) q_store(h, p.hq, p.hs, row, p.nb * 128, p.RpH, kb, l, live);     // (f(0) = 0: the padding stays zero codes)
+    else if (live) h_store8<VEC>(p.h + row * p.H, c, p.H, h);
+  }
+}
+
+// ----------------------------------------------------------------------------------------------- activation, backward
+template <int ACT, bool VEC>
+__global__ __launch_bounds__(256) void ea_act_use_kernel(ActParams p) {
+  constexpr int G = ACT == EA_ACT_GEGLU ? 2 : 1;
+  const int l = threadIdx.x & 15;
+  const long long rt = blockIdx.x / p.gx;
+  const long long row = rt * 16 + (threadIdx.x >> 4);
+  const int kb0 = (blockIdx.x - (int)(rt * p.gx)) * Q_KB;
+  if (row >= p.M) return;
+#pragma unroll
+  for (int u = 0; u < Q_KB; ++u) {
+    const int kb = kb0 + u, c = kb * 128 + l * 8;
+    if (kb >= p.nb) break;
+    float z[G][8], d[8], o[G][8];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      q_decode8(p.zq + (row * G + g) * p.nb * 128 + c, ea_fp8_scale(p.zs[kb * p.RpZ + row * G + g]), z[g]);
+    h_load8<VEC>(p.dh + row * p.H, c, p.H, d);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (G == 2) {
+        float P, xp;
+        gelu_parts(z[1][j], P, xp);
+        o[0][j] = d[j] * (z[1][j] * P);
+        o[1][j] = d[j] * z[0][j] * (P + xp);
+      } else o[0][j] = d[j] * act_slope<ACT>(z[0][j]);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) h_store8<VEC>(p.dz + (row * G + g) * p.H, c, p.H, o[g]);
+  }
+}
+
+bool al16(const void* a, const void* b = nullptr, const void* c = nullptr) {
+  return ((((uintptr_t)a) | ((uintptr_t)b) | ((uintptr_t)c)) & 15) == 0;
+}
+// workgroups of 16 rows x Q_KB blocks, column tiles fastest; 0: more than a grid holds
+unsigned q_grid(long long rows, int nb, int& gx) {
+  gx = (nb + Q_KB - 1) / Q_KB;
+  const long long g = (rows + 15) / 16 * gx;
+  return g > 0x7fffffffll ? 0u : (unsigned)g;
+}
+
+}  // namespace
+
+extern "C" int ea_quantize_fp8(const void* x, int in_f32, void* q, unsigned char* scale, long long rows, int cols, void* stream) {
+  if (!x || !q || !scale) return EA_ERR_BAD_ARG;
+  if (rows <= 0 || cols <= 0 || cols > (1 << 24)) return EA_ERR_BAD_SHAPE;
+  if (!al16(q)) return EA_ERR_BAD_ARG;
+  int gx;
+  const int nb = ea_fp8_blocks(cols);
+  const unsigned grid = q_grid(rows, nb, gx);
+  if (!grid) return EA_ERR_BAD_SHAPE;
+  const bool vec = (cols & 7) == 0 && al16(x);
+  auto k = in_f32 ? (vec ? ea_quant_rows_kernel<true, true> : ea_quant_rows_kernel<true, false>)
+                  : (vec ? ea_quant_rows_kernel<false, true> : ea_quant_rows_kernel<false, false>);
+  EA_LAUNCH(k, dim3(grid), dim3(256), 0, stream, x, (uint8_t*)q, scale, rows, cols, nb, ea_fp8_scale_pitch(rows), gx);
+  return ea_launch_status();
+}
+
+extern "C" int ea_quantize_fp8_weight(const void* w, int in_f32, void* q, unsigned char* scale, int N, int K, void* stream) {
+  if (!w || !q || !scale) return EA_ERR_BAD_ARG;
+  if (N <= 0 || K <= 0 || N > (1 << 22) || K > (1 << 24)) return EA_ERR_BAD_SHAPE;
+  if (!al16(q)) return EA_ERR_BAD_ARG;
+  const bool vec = (K & 7) == 0 && al16(w);
+  auto k = in_f32 ? (vec ? ea_quant_weight_kernel<true, true> : ea_quant_weight_kernel<true, false>)
+                  : (vec ? ea_quant_weight_kernel<false, true> : ea_quant_weight_kernel<false, false>);
+  EA_LAUNCH(k, dim3(ea_fp8_blocks(K), (N + 127) / 128), dim3(256), 64, stream, w, (uint8_t*)q, scale, N, K, ea_fp8_blocks(K));
+  return ea_launch_status();
+}
+
+extern "C" int ea_dequantize_fp8(const void* q, const unsigned char* scale, int block_rows, void* out, int out_f32, long long rows, int cols,
+                                 void* stream) {
+  if (!q || !scale || !out) return EA_ERR_BAD_ARG;
+  if (rows <= 0 || cols <= 0 || cols > (1 << 24)) return EA_ERR_BAD_SHAPE;
+  if (!al16(q) || (block_rows != 1 && block_rows != 128)) return EA_ERR_BAD_ARG;
+  int gx;
+  const int nb = ea_fp8_blocks(cols);
+  const unsigned grid = q_grid(rows, nb, gx);
+  if (!grid) return EA_ERR_BAD_SHAPE;
+  const bool vec = (cols & 7) == 0 && al16(out);
+  auto k = out_f32 ? (vec ? ea_dequant_kernel<true, true> : ea_dequant_kernel<true, false>)
+                   : (vec ? ea_dequant_kernel<false, true> : ea_dequant_kernel<false, false>);
+  EA_LAUNCH(k, dim3(grid), dim3(256), 0, stream, (const uint8_t*)q, scale, out, rows, cols, nb,
+            block_rows == 1 ? ea_fp8_scale_pitch(rows) : (rows + 127) / 128, block_rows == 1 ? 0 : 7, gx);
+  return ea_launch_status();
+}
+
+static int act_params(ActParams& p, int act, long long M, int H, unsigned& grid) {
+  if (act != EA_ACT_SILU && act != EA_ACT_GELU && act != EA_ACT_GEGLU) return EA_ERR_BAD_ARG;
+  if (M <= 0 || H <= 0 || H > (1 << 24)) return EA_ERR_BAD_SHAPE;
+  memset(&p, 0, sizeof(p));
+  p.M = M; p.H = H; p.nb = ea_fp8_blocks(H);
+  p.RpH = ea_fp8_scale_pitch(M);
+  p.RpZ = ea_fp8_scale_pitch(act == EA_ACT_GEGLU ? 2 * M : M);
+  grid = q_grid(M, p.nb, p.gx);
+  return grid ? EA_OK : EA_ERR_BAD_SHAPE;
+}
+
+extern "C" int ea_activation_fp8(const void* z, int act, void* h, void* hq, unsigned char* hscale, void* zq, unsigned char* zscale, long long M,
+                                 int H, void* stream) {
+  if (!z || !zq || !zscale || (!h == !hq) || (hq && !hscale)) return EA_ERR_BAD_ARG;
+  ActParams p;
+  unsigned grid;
+  const int st = act_params(p, act, M, H, grid);
+  if (st != EA_OK) return st;
+  if (!al16(zq, hq)) return EA_ERR_BAD_ARG;
+  p.z = (const f16*)z; p.h = (f16*)h; p.hq = (uint8_t*)hq; p.hs = hscale; p.zq = (uint8_t*)zq; p.zs = zscale;
+  const bool vec = (H & 7) == 0 && al16(z, h), o8 = hq != nullptr;
+#define EA_ACT_PICK(A) (vec ? (o8 ? ea_act_save_kernel<A, true, true> : ea_act_save_kernel<A, true, false>) \
+                            : (o8 ? ea_act_save_kernel<A, false, true> : ea_act_save_kernel<A, false, false>))
+  auto k = act == EA_ACT_SILU ? EA_ACT_PICK(EA_ACT_SILU) : act == EA_ACT_GELU ? EA_ACT_PICK(EA_ACT_GELU) : EA_ACT_PICK(EA_ACT_GEGLU);
+#undef EA_ACT_PICK
+  EA_LAUNCH(k, dim3(grid), dim3(256), 0, stream, p);
+  return ea_launch_status();
+}
+
+extern "C" int ea_activation_fp8_bwd(const void* dh, const void* zq, const unsigned char* zscale, int act, void* dz, long long M, int H,
+                                     void* stream) {
+  if (!dh || !zq || !zscale || !dz) return EA_ERR_BAD_ARG;
+  ActParams p;
+  unsigned grid;
+  const int st = act_params(p, act, M, H, grid);
+  if (st != EA_OK) return st;
+  if (!al16(zq)) return EA_ERR_BAD_ARG;
+  p.dh = (const f16*)dh; p.dz = (f16*)dz; p.zq = (uint8_t*)const_cast<void*>(zq); p.zs = const_cast<unsigned char*>(zscale);
+  const bool vec = (H & 7) == 0 && al16(dh, dz);
+  auto k = act == EA_ACT_SILU ? (vec ? ea_act_use_kernel<EA_ACT_SILU, true> : ea_act_use_kernel<EA_ACT_SILU, false>)
+         : act == EA_ACT_GELU ? (vec ? ea_act_use_kernel<EA_ACT_GELU, true> : ea_act_use_kernel<EA_ACT_GELU, false>)
+                              : (vec ? ea_act_use_kernel<EA_ACT_GEGLU, true> : ea_act_use_kernel<EA_ACT_GEGLU, false>);
+  EA_LAUNCH(k, dim3(grid), dim3(256), 0, stream, p);
+  return ea_launch_status();
+}

@@ -1,0 +1,386 @@
+// ea_train.hip -- LayerNorm for training: the forward pass that keeps its row statistics, and the backward pass with the
+// reductions of the weight's and the bias's gradients.
+//
+//   forward    mu = mean(x), r = (mean((x - mu)^2) + eps)^-1/2 per row;  y = (x - mu) r gamma + beta
+//   backward   n = (x - mu) r,  g = dy gamma:
+//              dx = r (g - mean(g) - n mean(g n)) [+ residual],   dgamma = sum_rows dy n,   dbeta = sum_rows dy
+// All sums and statistics are fp32; the variance is the centred one (two passes over registers).  x is fp16, fp32 or an 8-bit
+// tensor (ea_fp8.h); the forward's y is fp16 or goes straight into the 8-bit format.
+//
+// Both passes read every operand once and are bound by HBM.  A row belongs to LPR lanes (8 ... 64: a 320-wide row is 40 16-byte
+// vectors, which would leave 24 of 64 lanes idle), so a wave holds 64 / LPR rows whole in registers; the row sums are DPP steps.
+// The column sums stay in registers over all rows that a wave visits (a lane always owns the same columns), are joined over the
+// workgroup in LDS once, written as one partial per workgroup and joined by a second launch in a fixed order: no atomics, so a
+// run repeats bit for bit.
+#include "ea_fp8.h"
+#include "../../include/editanything_hip.h"
+
+namespace {
+
+enum { XK_F16 = 0, XK_F32 = 1, XK_FP8 = 2 };
+
+// VEC consecutive values of one row (VEC = 8: 16-byte loads, C a multiple of 8; VEC = 1: any C)
+template <int XK, int VEC>
+__device__ __forceinline__ void ld_row(const void* x, const uint8_t* scale, long long row, int pitch, long long spitch, int c, float* v) {
+  if constexpr (XK == XK_F16) {
+    const f16* p = (const f16*)x + row * pitch + c;
+    if constexpr (VEC == 8) {
+      const f16x8 h = ea_ld8(p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+    } else v[0] = (float)*p;
+  } else if constexpr (XK == XK_F32) {
+    const float* p = (const float*)x + row * pitch + c;
+    if constexpr (VEC == 8) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    } else v[0] = *p;
+  } else {
+    const uint8_t* p = (const uint8_t*)x + row * pitch + c;
+    const float s = ea_fp8_scale(scale[(long long)(c >> 7) * spitch + row]);
+    if constexpr (VEC == 8) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+      ea_fp8_unpack4(w[0], v);
+      ea_fp8_unpack4(w[1], v + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= s;
+    } else {
+      float t[4];
+      ea_fp8_unpack4(*p, t);
+      v[0] = t[0] * s;
+    }
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void ld_f32(const float* p, float* v) {
+  if constexpr (VEC == 8) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+  } else v[0] = *p;
+}
+
+// ------------------------------------------------------------------------------------------------------------ forward
+struct LnTrainParams {
+  const void* x; const float* gamma; const float* beta;
+  f16* y;                              // fp16 output, or NULL
+  uint8_t* q; uint8_t* scale;          // 8-bit output
+  float* stats;                        // [M][2]: mean, 1 / sigma
+  int M, C, Kp; long long Rp;
+  float eps;
+};
+
+template <int XK, int VEC, int LPR, int NV, bool OUT8>
+__global__ __launch_bounds__(256) void ea_ln_train_kernel(LnTrainParams p) {
+  constexpr int RPW = 64 / LPR;
+  const int lane = threadIdx.x & 63, sub = lane / LPR, l = lane % LPR;
+  const int row = (blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW + sub;
+  const int r = row < p.M ? row : p.M - 1;
+  float x[NV][VEC];
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * VEC;
+    if (c < p.C) ld_row<XK, VEC>(p.x, nullptr, r, p.C, 0, c, x[i]);
+    else
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[i][j] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s += x[i][j];
+  }
+  const float mean = ea_group_sum<LPR>(s) / (float)p.C;
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float d = c < p.C ? x[i][j] - mean : 0.0f;
+      q += d * d;
+    }
+  }
+  const float rstd = 1.0f / sqrtf(ea_group_sum<LPR>(q) / (float)p.C + p.eps);
+  if (row < p.M && l == 0) *reinterpret_cast<f32x2*>(p.stats + 2ll * row) = f32x2{mean, rstd};
+  float bmax[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * VEC;
+    bmax[i] = 0.0f;
+    if (c < p.C) {
+      float ga[VEC], be[VEC];
+      ld_f32<VEC>(p.gamma + c, ga);
+      ld_f32<VEC>(p.beta + c, be);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        x[i][j] = (x[i][j] - mean) * rstd * ga[j] + be[j];
+        bmax[i] = fmaxf(bmax[i], ea_finite_abs(x[i][j]));
+      }
+      if (!OUT8 && row < p.M) {
+        f16* o = p.y + (long long)row * p.C + c;
+        if constexpr (VEC == 8) {
+          f16x8 h;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] = (f16)x[i][j];
+          ea_st8(o, h);
+        } else *o = (f16)x[i][0];
+      }
+    }
+  }
+  if constexpr (OUT8) {
+    // a block of 128 columns: 16 lanes of one vector (LPR >= 16), or PAIR vectors of the whole group (8 lanes; 64 scalars)
+    constexpr int PAIR = (VEC == 1 || LPR == 8) ? 2 : 1;
+    constexpr int GRP = VEC == 1 ? 64 : (LPR < 16 ? LPR : 16);
+    static_assert(NV % PAIR == 0, "a block's vectors come in pairs");
+#pragma unroll
+    for (int i = 0; i < NV; i += PAIR) {
+      float m = bmax[i];
+      if (PAIR == 2) m = fmaxf(m, bmax[i + PAIR - 1]);
+      m = ea_group_max<GRP>(m);
+      const int e = ea_fp8_exp_byte(m);
+      const float inv = ea_fp8_inv_scale(e);
+#pragma unroll
+      for (int u = 0; u < PAIR; ++u) {
+        const int c = (l + LPR * (i + u)) * VEC;
+        if (row < p.M && c < p.Kp) {
+          uint8_t* o = p.q + (long long)row * p.Kp + c;
+          if constexpr (VEC == 8) *reinterpret_cast<u32x2*>(o) = ea_fp8_encode8(x[i + u], inv);
+          else *o = (uint8_t)ea_fp8_pack4(ea_fp8_prep(x[i + u][0], inv), 0.0f, 0.0f, 0.0f);
+          if ((c & 127) == 0) p.scale[(long long)(c >> 7) * p.Rp + row] = (uint8_t)e;
+        }
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------- backward
+struct LnBwdParams {
+  const f16* dy; const void* x; const uint8_t* x_scale; const float* stats; const float* gamma;
+  const void* residual; void* dx; int dx_f32;          // residual and dx share a type
+  float* part;                         // [gridDim.x][2][C]
+  int M, C, xpitch; long long xspitch;
+};
+
+template <int XK, int VEC, int LPR, int NV>
+__global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
+  constexpr int RPW = 64 / LPR;
+  constexpr bool KEEP = NV <= 24;      // more scalars per lane than that do not fit in registers twice: the row is read again (from L2)
+  EA_SMEM(smem);
+  float* red = reinterpret_cast<float*>(smem);      // [4][C]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, l = lane % LPR;
+  float ga[NV][VEC], ag[NV][VEC], ab[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) ga[i][j] = ag[i][j] = ab[i][j] = 0.0f;
+    if (c < p.C) ld_f32<VEC>(p.gamma + c, ga[i]);
+  }
+  const float inv_c = 1.0f / (float)p.C;
+  const long long stride = (long long)gridDim.x * 4 * RPW;
+  for (long long base = ((long long)blockIdx.x * 4 + wave) * RPW; base < p.M; base += stride) {
+    const long long row = base + sub;
+    const bool live = row < p.M;
+    const long long r = live ? row : p.M - 1;
+    const f32x2 st = *reinterpret_cast<const f32x2*>(p.stats + 2 * r);
+    float n[KEEP ? NV : 1][VEC], g[KEEP ? NV : 1][VEC];
+    float s1 = 0.0f, s2 = 0.0f;
+    auto load = [&](int c, float* nv, float* gv) {
+      if (c < p.C) {
+        ld_row<XK, VEC>(p.x, p.x_scale, r, p.xpitch, p.xspitch, c, nv);
+        ld_row<XK_F16, VEC>(p.dy, nullptr, r, p.C, 0, c, gv);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) nv[j] = gv[j] = 0.0f;
+      }
+    };
+    if (KEEP)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load((l + LPR * i) * VEC, n[KEEP ? i : 0], g[KEEP ? i : 0]);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (l + LPR * i) * VEC, k = KEEP ? i : 0;
+      if (!KEEP) load(c, n[k], g[k]);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float d = live && c < p.C ? g[k][j] : 0.0f;      // (a row or column that is not there adds nothing, whatever was read)
+        n[k][j] = live && c < p.C ? (n[k][j] - st[0]) * st[1] : 0.0f;
+        ag[i][j] += d * n[k][j];
+        ab[i][j] += d;
+        g[k][j] = d * ga[i][j];
+        s1 += g[k][j];
+        s2 += g[k][j] * n[k][j];
+      }
+    }
+    s1 = ea_group_sum<LPR>(s1) * inv_c;
+    s2 = ea_group_sum<LPR>(s2) * inv_c;
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (l + LPR * i) * VEC, k = KEEP ? i : 0;
+        if (c >= p.C) continue;
+        if (!KEEP) {
+          load(c, n[k], g[k]);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            n[k][j] = (n[k][j] - st[0]) * st[1];
+            g[k][j] *= ga[i][j];
+          }
+        }
+        float o[VEC], res[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          o[j] = st[1] * (g[k][j] - s1 - n[k][j] * s2);
+          res[j] = 0.0f;
+        }
+        if (p.dx_f32) {
+          if (p.residual) ld_row<XK_F32, VEC>(p.residual, nullptr, row, p.C, 0, c, res);
+          float* d = (float*)p.dx + row * p.C + c;
+          if constexpr (VEC == 8) {
+            *reinterpret_cast<f32x4*>(d) = f32x4{o[0] + res[0], o[1] + res[1], o[2] + res[2], o[3] + res[3]};
+            *reinterpret_cast<f32x4*>(d + 4) = f32x4{o[4] + res[4], o[5] + res[5], o[6] + res[6], o[7] + res[7]};
+          } else *d = o[0] + res[0];
+        } else {
+          if (p.residual) ld_row<XK_F16, VEC>(p.residual, nullptr, row, p.C, 0, c, res);
+          f16* d = (f16*)p.dx + row * p.C + c;
+          if constexpr (VEC == 8) {
+            f16x8 h;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = (f16)(o[j] + res[j]);
+            ea_st8(d, h);
+          } else *d = (f16)(o[0] + res[0]);
+        }
+      }
+    }
+  }
+  // column sums: the wave's rows, then the four waves, in a fixed order
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (half) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (l + LPR * i) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float v = half ? ab[i][j] : ag[i][j];
+#pragma unroll
+        for (int m = LPR; m < 64; m <<= 1) v += ea_shfl_xor(v, m);
+        if (sub == 0 && c < p.C) red[wave * p.C + c + j] = v;
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.C; c += 256)
+      p.part[((long long)blockIdx.x * 2 + half) * p.C + c] = (red[c] + red[p.C + c]) + (red[2 * p.C + c] + red[3 * p.C + c]);
+  }
+}
+
+// out[c] = sum_g part[g][c] in a fixed order: a workgroup owns 32 columns, 32 lanes of partials each
+__global__ __launch_bounds__(1024) void ea_ln_join_kernel(const float* part, float* out, int G, int cols) {
+  EA_SMEM(smem);
+  float* red = reinterpret_cast<float*>(smem);      // [32][33]
+  const int cx = threadIdx.x & 31, gy = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + cx;
+  float s = 0.0f;
+  if (c < cols)
+#pragma unroll 8
+    for (int g = gy; g < G; g += 32) s += part[(long long)g * cols + c];
+  red[gy * 33 + cx] = s;
+  __syncthreads();
+  for (int h = 16; h > 0; h >>= 1) {
+    if (gy < h) red[gy * 33 + cx] += red[(gy + h) * 33 + cx];
+    __syncthreads();
+  }
+  if (gy == 0 && c < cols) out[c] = red[cx];
+}
+
+bool ln_vec(int C, const void* a, const void* b, const void* c, const void* d, const void* e, const void* f) {
+  return (C & 7) == 0 && ((((uintptr_t)a) | ((uintptr_t)b) | ((uintptr_t)c) | ((uintptr_t)d) | ((uintptr_t)e) | ((uintptr_t)f)) & 15) == 0;
+}
+// lanes per row: the fewest that hold a row in at most 5 (8 lanes: 6) vectors of 8 columns; scalars always take the wave
+int ln_lanes(int C, bool vec) { return !vec ? 64 : C <= 384 ? 8 : C <= 640 ? 16 : C <= 1280 ? 32 : 64; }
+
+template <int XK, bool OUT8>
+int ln_train_launch(const LnTrainParams& p, bool vec, void* stream) {
+  void (*k)(LnTrainParams);
+  const int lpr = ln_lanes(p.C, vec);
+  if (vec) {
+    k = lpr == 8 ? ea_ln_train_kernel<XK, 8, 8, 6, OUT8> : lpr == 16 ? ea_ln_train_kernel<XK, 8, 16, 5, OUT8>
+      : lpr == 32 ? ea_ln_train_kernel<XK, 8, 32, 5, OUT8> : p.C <= 2560 ? ea_ln_train_kernel<XK, 8, 64, 5, OUT8>
+      : ea_ln_train_kernel<XK, 8, 64, 8, OUT8>;
+  } else {
+    k = p.C <= 512 ? ea_ln_train_kernel<XK, 1, 64, 8, OUT8> : p.C <= 1536 ? ea_ln_train_kernel<XK, 1, 64, 24, OUT8>
+      : ea_ln_train_kernel<XK, 1, 64, 64, OUT8>;
+  }
+  const int rows = 4 * (64 / lpr);
+  EA_LAUNCH(k, dim3((p.M + rows - 1) / rows), dim3(256), 0, stream, p);
+  return ea_launch_status();
+}
+
+constexpr int LN_MAX_WG = 512;
+int ln_bwd_grid(int M, int C) {            // the same for both paths of a width: the workspace does not depend on alignment
+  const int rows = 4 * (64 / ln_lanes(C, (C & 7) == 0));
+  const int g = (M + rows - 1) / rows;
+  return g < LN_MAX_WG ? g : LN_MAX_WG;
+}
+
+template <int XK>
+int ln_bwd_launch(const LnBwdParams& p, bool vec, int grid, void* stream) {
+  void (*k)(LnBwdParams);
+  const int lpr = ln_lanes(p.C, vec);
+  if (vec) {
+    k = lpr == 8 ? ea_ln_bwd_kernel<XK, 8, 8, 6> : lpr == 16 ? ea_ln_bwd_kernel<XK, 8, 16, 5>
+      : lpr == 32 ? ea_ln_bwd_kernel<XK, 8, 32, 5> : p.C <= 2560 ? ea_ln_bwd_kernel<XK, 8, 64, 5>
+      : ea_ln_bwd_kernel<XK, 8, 64, 8>;
+  } else {
+    k = p.C <= 512 ? ea_ln_bwd_kernel<XK, 1, 64, 8> : p.C <= 1536 ? ea_ln_bwd_kernel<XK, 1, 64, 24>
+      : ea_ln_bwd_kernel<XK, 1, 64, 64>;
+  }
+  const int smem = 4 * p.C * (int)sizeof(float);
+  ea_allow_big_lds(k, smem);
+  EA_LAUNCH(k, dim3(grid), dim3(256), smem, stream, p);
+  return ea_launch_status();
+}
+
+}  // namespace
+
+extern "C" int ea_layernorm_train(const void* x, int in_f32, const float* gamma, const float* beta, float eps, void* y, void* q,
+                                  unsigned char* scale, float* stats, int M, int C, void* stream) {
+  if (!x || !gamma || !beta || !stats || (!y == !q) || (q && !scale)) return EA_ERR_BAD_ARG;
+  if (M <= 0 || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
+  if (((uintptr_t)stats & 7) || ((uintptr_t)q & 15)) return EA_ERR_BAD_ARG;
+  LnTrainParams p;
+  p.x = x; p.gamma = gamma; p.beta = beta; p.y = (f16*)y; p.q = (uint8_t*)q; p.scale = scale; p.stats = stats;
+  p.M = M; p.C = C; p.Kp = ea_fp8_blocks(C) * EA_FP8_BLOCK; p.Rp = ea_fp8_scale_pitch(M); p.eps = eps;
+  const bool vec = ln_vec(C, x, gamma, beta, y, nullptr, nullptr);
+  if (in_f32) return q ? ln_train_launch<XK_F32, true>(p, vec, stream) : ln_train_launch<XK_F32, false>(p, vec, stream);
+  return q ? ln_train_launch<XK_F16, true>(p, vec, stream) : ln_train_launch<XK_F16, false>(p, vec, stream);
+}
+
+extern "C" size_t ea_layernorm_bwd_workspace_bytes(int M, int C) {
+  if (M <= 0 || C <= 0 || C > 4096) return 0;
+  return (size_t)ln_bwd_grid(M, C) * 2 * C * sizeof(float);
+}
+
+extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const unsigned char* x_scale, const float* stats,
+                                const float* gamma, const void* residual, void* dx, int dx_f32, float* dgamma_dbeta, int M, int C,
+                                void* workspace, size_t ws_bytes, void* stream) {
+  if (!dy || !x || !stats || !gamma || !dx || !dgamma_dbeta || !workspace || (x_kind == XK_FP8 && !x_scale)) return EA_ERR_BAD_ARG;
+  if (x_kind < XK_F16 || x_kind > XK_FP8) return EA_ERR_BAD_ARG;
+  if (M <= 0 || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
+  if (((uintptr_t)stats & 7) || ((uintptr_t)workspace & 3)) return EA_ERR_BAD_ARG;
+  if (ws_bytes < ea_layernorm_bwd_workspace_bytes(M, C)) return EA_ERR_WORKSPACE;
+  LnBwdParams p;
+  p.dy = (const f16*)dy; p.x = x; p.x_scale = x_scale; p.stats = stats; p.gamma = gamma; p.residual = residual; p.dx = dx; p.dx_f32 = dx_f32;
+  p.part = (float*)workspace; p.M = M; p.C = C;
+  p.xpitch = x_kind == XK_FP8 ? ea_fp8_blocks(C) * EA_FP8_BLOCK : C;
+  p.xspitch = ea_fp8_scale_pitch(M);
+  const bool vec = ln_vec(C, dy, x, gamma, residual, dx, nullptr);
+  const int grid = ln_bwd_grid(M, C);
+  const int st = x_kind == XK_F16 ? ln_bwd_launch<XK_F16>(p, vec, grid, stream) : x_kind == XK_F32 ? ln_bwd_launch<XK_F32>(p, vec, grid, stream)
+                                  : ln_bwd_launch<XK_FP8>(p, vec, grid, stream);
+  if (st != EA_OK) return st;
+  auto k = ea_ln_join_kernel;
+  EA_LAUNCH(k, dim3((2 * C + 31) / 32), dim3(1024), 32 * 33 * sizeof(float), stream, (const float*)workspace, dgamma_dbeta, grid, 2 * C);
+  return ea_launch_status();
+}

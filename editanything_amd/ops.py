@@ -976,3 +976,248 @@ def add_f16(a, b):
     out = torch.empty_like(a)
     L.check(_lib().ea_add_f16(_p(a), _p(b), _p(out), a.numel(), _stream()), "ea_add_f16")
     return out
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit training operators
+# LayerNorm with its backward pass, activations whose input is kept in 8 bits for the backward pass, the product of 8-bit operands and
+# the weight gradient from an 8-bit input: what a transformer block (LayerNorm -> Linear -> activation -> Linear + residual) needs to be
+# trained with its activations held in 8 bits.  Every operator is a plain function; the caller keeps what the backward pass takes.
+# Outputs and scratch come from torch's allocator on the current stream of the operands' device, never from the shared per-thread
+# workspace, so calls on several streams and in several captured graphs do not meet.
+FP8_BLOCK = 128
+
+
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _check_fp8(dev, **tensors):
+    """Device and layout of one 8-bit operator's operands: all dense, on one MI355X."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"editanything_amd ops run on the MI355X only ({name} is on {t.device})")
+        _need(t.device == dev, f"{name} is on {t.device}, the other operands on {dev}")
+        _need(t.is_contiguous(), f"{name} must be contiguous, got strides {tuple(t.stride())} for shape {tuple(t.shape)}")
+
+
+def _run(dev, what, fn, *args):
+    """One C call on `dev`'s current stream (the device is switched for the launch where it is not the current one)."""
+    if dev.index == torch.cuda.current_device():
+        L.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
+    else:
+        with torch.cuda.device(dev):
+            L.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
+
+
+class Fp8Tensor:
+    """Rows in 8 bits: e4m3 codes with one power-of-two scale for each block of 128 columns (include/editanything_hip.h).
+
+    q      float8_e4m3fn [rows, 128 * blocks]: the codes, a row's last block padded with zeros
+    scale  uint8: the exponent byte E + 127 of each block; a code stands for code * 2^E.
+           rows:   [blocks, rows rounded up to 16]      (`quantize_fp8`; the bytes behind the last row are never used)
+           weight: [blocks, ceil(rows / 128)], one exponent for 128 x 128      (`quantize_fp8_weight`)
+    cols   the columns that are there;  shape: the logical shape (leading dimensions x cols)."""
+    __slots__ = ("q", "scale", "cols", "rows", "shape", "block_rows")
+
+    def __init__(self, q, scale, cols, shape=None):
+        nb = -(-cols // FP8_BLOCK)
+        _need(q.dim() == 2 and q.dtype == torch.float8_e4m3fn and cols > 0 and q.shape[1] == nb * FP8_BLOCK,
+              f"Fp8Tensor: q must be float8_e4m3fn [rows, {nb * FP8_BLOCK}] for {cols} columns, got {q.dtype} {tuple(q.shape)}")
+        rows = q.shape[0]
+        rp = (rows + 15) // 16 * 16
+        _need(scale.dtype == torch.uint8 and scale.dim() == 2 and scale.shape[0] == nb and scale.shape[1] in (rp, -(-rows // 128)),
+              f"Fp8Tensor: scale must be uint8 [{nb}, {rp}] (rows) or [{nb}, {-(-rows // 128)}] (weight), got {scale.dtype} {tuple(scale.shape)}")
+        self.q, self.scale, self.cols, self.rows = q, scale, cols, rows
+        self.block_rows = 1 if scale.shape[1] == rp else FP8_BLOCK
+        self.shape = torch.Size((rows, cols)) if shape is None else torch.Size(shape)
+        _need(self.shape[-1] == cols and self.shape.numel() == rows * cols, f"Fp8Tensor: shape {tuple(self.shape)} is not {rows} rows of {cols}")
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def dequantize(self, dtype=torch.float16):
+        return dequantize_fp8(self, dtype)
+
+
+def _fp8_empty(rows, cols, dev, shape=None):
+    nb = -(-cols // FP8_BLOCK)
+    return Fp8Tensor(torch.empty((rows, nb * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=dev),
+                     torch.empty((nb, (rows + 15) // 16 * 16), dtype=torch.uint8, device=dev), cols, shape)
+
+
+def _rows_of(name, x, dtypes):
+    _need(torch.is_tensor(x) and x.dtype in dtypes, f"{name} must be a tensor of {' or '.join(str(d) for d in dtypes)}"
+          f", got {x.dtype if torch.is_tensor(x) else type(x).__name__}")
+    _need(x.dim() >= 1 and x.shape[-1] > 0, f"{name} needs a last dimension, got shape {tuple(x.shape)}")
+    return x.numel() // x.shape[-1], x.shape[-1]
+
+
+def _rows_fp8(name, t):
+    _need(isinstance(t, Fp8Tensor) and t.block_rows == 1, f"{name} must be an Fp8Tensor of rows (quantize_fp8)")
+
+
+def quantize_fp8(x):
+    """fp16 / fp32 [..., C] -> Fp8Tensor, one scale for each row and block of 128 columns.  NaN and infinities become NaN codes."""
+    rows, cols = _rows_of("x", x, (torch.float16, torch.float32))
+    _check_fp8(x.device, x=x)
+    t = _fp8_empty(rows, cols, x.device, x.shape)
+    if rows:
+        _run(x.device, "ea_quantize_fp8", _lib().ea_quantize_fp8, _p(x), int(x.dtype == torch.float32), _p(t.q), _p(t.scale), rows, cols)
+    return t
+
+
+def quantize_fp8_weight(w):
+    """fp16 / fp32 weight [N, K] -> Fp8Tensor, one scale for 128 x 128.  The blocks are square, so `w.t().contiguous()` quantises to the
+    same values: that is the operand of the input gradient, dx = gemm_fp8(quantize_fp8(dy), quantize_fp8_weight(w.t().contiguous()))."""
+    _need(torch.is_tensor(w) and w.dim() == 2, "quantize_fp8_weight: a weight is [N, K]")
+    n, k = _rows_of("w", w, (torch.float16, torch.float32))
+    _need(n > 0, "quantize_fp8_weight: the weight has no rows")
+    _check_fp8(w.device, w=w)
+    nb = -(-k // FP8_BLOCK)
+    t = Fp8Tensor(torch.empty((n, nb * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=w.device),
+                  torch.empty((nb, -(-n // 128)), dtype=torch.uint8, device=w.device), k)
+    _run(w.device, "ea_quantize_fp8_weight", _lib().ea_quantize_fp8_weight, _p(w), int(w.dtype == torch.float32), _p(t.q), _p(t.scale), n, k)
+    return t
+
+
+def dequantize_fp8(t, dtype=torch.float16):
+    """The values an Fp8Tensor stands for, fp16 (rounded) or fp32 (exact); beyond the type's range infinite."""
+    _need(isinstance(t, Fp8Tensor), "dequantize_fp8 takes an Fp8Tensor")
+    _need(dtype in (torch.float16, torch.float32), f"dequantize_fp8: fp16 or fp32, not {dtype}")
+    _check_fp8(t.device, q=t.q, scale=t.scale)
+    out = torch.empty(t.shape, dtype=dtype, device=t.device)
+    if t.rows:
+        _run(t.device, "ea_dequantize_fp8", _lib().ea_dequantize_fp8, _p(t.q), _p(t.scale), t.block_rows, _p(out), int(dtype == torch.float32),
+             t.rows, t.cols)
+    return out
+
+
+def layernorm_train(x, gamma, beta, eps=1e-5, fp8=False):
+    """LayerNorm over the last dimension (at most 4096) that keeps its statistics for `layernorm_backward`.
+    x fp16 / fp32 [..., C]; gamma, beta fp32 [C].  -> (y, stats): y fp16, or with `fp8` an Fp8Tensor (the next product's operand and its
+    weight gradient's input, written in the same pass); stats fp32 [rows, 2] = (mean, 1 / sigma)."""
+    M, Cc = _rows_of("x", x, (torch.float16, torch.float32))
+    _need(Cc <= 4096, f"layernorm_train: at most 4096 columns, got {Cc}")
+    for name, t in (("gamma", gamma), ("beta", beta)):
+        _need(torch.is_tensor(t) and t.dtype == torch.float32 and t.shape == (Cc,), f"layernorm_train: {name} must be fp32 [{Cc}]")
+    _check_fp8(x.device, x=x, gamma=gamma, beta=beta)
+    stats = torch.empty((M, 2), dtype=torch.float32, device=x.device)
+    y = _fp8_empty(M, Cc, x.device, x.shape) if fp8 else torch.empty(x.shape, dtype=torch.float16, device=x.device)
+    if M:
+        _run(x.device, "ea_layernorm_train", _lib().ea_layernorm_train, _p(x), int(x.dtype == torch.float32), _p(gamma), _p(beta), float(eps),
+             None if fp8 else _p(y), _p(y.q) if fp8 else None, _p(y.scale) if fp8 else None, _p(stats), M, Cc)
+    return y, stats
+
+
+def layernorm_backward(dy, x, stats, gamma, residual=None):
+    """Backward pass of `layernorm_train`: dy fp16 [..., C]; x the forward's input, fp16, fp32 or an Fp8Tensor of it (kept in 8 bits in
+    place of x); stats as the forward left them.  -> (dx, dgamma, dbeta): dx has x's type (fp16 for an Fp8Tensor) plus `residual` (the
+    gradient that bypasses the norm, dx's type); dgamma, dbeta fp32 [C], summed in a fixed order."""
+    M, Cc = _rows_of("dy", dy, (torch.float16,))
+    q8 = isinstance(x, Fp8Tensor)
+    if q8:
+        _rows_fp8("x", x)
+    else:
+        _rows_of("x", x, (torch.float16, torch.float32))
+    _need(x.shape == dy.shape, f"layernorm_backward: x {tuple(x.shape)} and dy {tuple(dy.shape)} must have one shape")
+    _need(Cc <= 4096, f"layernorm_backward: at most 4096 columns, got {Cc}")
+    out = torch.float16 if q8 else x.dtype
+    _need(torch.is_tensor(gamma) and gamma.dtype == torch.float32 and gamma.shape == (Cc,), f"layernorm_backward: gamma must be fp32 [{Cc}]")
+    _need(torch.is_tensor(stats) and stats.dtype == torch.float32 and stats.shape == (M, 2), f"layernorm_backward: stats must be fp32 [{M}, 2]")
+    if residual is not None:
+        _need(residual.dtype == out and residual.shape == dy.shape, f"layernorm_backward: residual must be {out} {tuple(dy.shape)}")
+    _check_fp8(dy.device, dy=dy, x=x.q if q8 else x, scale=x.scale if q8 else None, stats=stats, gamma=gamma, residual=residual)
+    dx = torch.empty(dy.shape, dtype=out, device=dy.device)
+    if not M:
+        grads = torch.zeros((2, Cc), dtype=torch.float32, device=dy.device)
+    else:
+        lib = _lib()
+        nbytes = lib.ea_layernorm_bwd_workspace_bytes(M, Cc)
+        buf = torch.empty((nbytes,), dtype=torch.uint8, device=dy.device)
+        grads = torch.empty((2, Cc), dtype=torch.float32, device=dy.device)
+        _run(dy.device, "ea_layernorm_bwd", lib.ea_layernorm_bwd, _p(dy), _p(x.q if q8 else x), 2 if q8 else int(x.dtype == torch.float32),
+             _p(x.scale) if q8 else None, _p(stats), _p(gamma), _p(residual), _p(dx), int(out == torch.float32), _p(grads), M, Cc, _p(buf), nbytes)
+    return dx, grads[0], grads[1]
+
+
+def _act_arg(act):
+    _need(act in (ACT_SILU, ACT_GELU, ACT_GEGLU), f"act must be ACT_SILU, ACT_GELU or ACT_GEGLU, not {act!r}")
+    return 2 if act == ACT_GEGLU else 1
+
+
+def activation_fp8(z, act, fp8=False):
+    """h = act(z) with z kept in 8 bits for `activation_fp8_backward`: one pass.  z fp16 [..., H] (ACT_SILU, ACT_GELU) or [..., 2 H] =
+    [value | gate] (ACT_GEGLU: h = value * gelu(gate)).  -> (h, saved): h fp16 [..., H], or with `fp8` an Fp8Tensor; saved: z as an
+    Fp8Tensor of rows of H (ACT_GEGLU: a row's value and gate halves one after the other, [..., 2, H])."""
+    g = _act_arg(act)
+    M, W = _rows_of("z", z, (torch.float16,))
+    _need(W % g == 0, f"activation_fp8: GEGLU needs an even last dimension, got {W}")
+    H = W // g
+    _check_fp8(z.device, z=z)
+    saved = _fp8_empty(M * g, H, z.device, z.shape if g == 1 else z.shape[:-1] + (2, H))
+    shape = z.shape[:-1] + (H,)
+    h = _fp8_empty(M, H, z.device, shape) if fp8 else torch.empty(shape, dtype=torch.float16, device=z.device)
+    if M:
+        _run(z.device, "ea_activation_fp8", _lib().ea_activation_fp8, _p(z), int(act), None if fp8 else _p(h), _p(h.q) if fp8 else None,
+             _p(h.scale) if fp8 else None, _p(saved.q), _p(saved.scale), M, H)
+    return h, saved
+
+
+def activation_fp8_backward(dh, saved, act):
+    """dz = dh * act'(z) with z decoded from `saved` (`activation_fp8`).  dh fp16 [..., H] -> dz fp16 [..., H] ([..., 2 H] for ACT_GEGLU)."""
+    g = _act_arg(act)
+    M, H = _rows_of("dh", dh, (torch.float16,))
+    _rows_fp8("saved", saved)
+    _need(saved.rows == M * g and saved.cols == H, f"activation_fp8_backward: dh {tuple(dh.shape)} does not belong to saved {tuple(saved.shape)}")
+    _check_fp8(dh.device, dh=dh, q=saved.q, scale=saved.scale)
+    dz = torch.empty(dh.shape[:-1] + (g * H,), dtype=torch.float16, device=dh.device)
+    if M:
+        _run(dh.device, "ea_activation_fp8_bwd", _lib().ea_activation_fp8_bwd, _p(dh), _p(saved.q), _p(saved.scale), int(act), _p(dz), M, H)
+    return dz
+
+
+def gemm_fp8(a, w, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=torch.float16, scale=1.0):
+    """out = residual + scale * act(a w^T + bias): a an Fp8Tensor of rows [..., K], w an Fp8Tensor weight [N, K]; bias fp32 [N]; act
+    ACT_NONE, ACT_SILU or ACT_GELU; residual fp16 or fp32 [..., N] (may be `out`); out fp16 or fp32."""
+    _rows_fp8("a", a)
+    _need(isinstance(w, Fp8Tensor) and w.block_rows == FP8_BLOCK, "gemm_fp8: w must be an Fp8Tensor weight (quantize_fp8_weight)")
+    _need(a.cols == w.cols, f"gemm_fp8: a has {a.cols} columns, w {w.cols}")
+    _need(act in (ACT_NONE, ACT_SILU, ACT_GELU), f"gemm_fp8: act must be ACT_NONE, ACT_SILU or ACT_GELU, not {act!r}")
+    M, N = a.rows, w.rows
+    shape = a.shape[:-1] + (N,)
+    if out is None:
+        _need(out_dtype in (torch.float16, torch.float32), f"gemm_fp8: out_dtype must be fp16 or fp32, not {out_dtype}")
+        out = torch.empty(shape, dtype=out_dtype, device=a.device)
+    for name, t, dts in (("out", out, (torch.float16, torch.float32)), ("residual", residual, (torch.float16, torch.float32))):
+        if t is not None:
+            _need(t.dtype in dts and t.shape == shape, f"gemm_fp8: {name} must be fp16 or fp32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if bias is not None:
+        _need(bias.dtype == torch.float32 and bias.shape == (N,), f"gemm_fp8: bias must be fp32 [{N}]")
+    _check_fp8(a.device, a=a.q, a_scale=a.scale, w=w.q, w_scale=w.scale, bias=bias, residual=residual, out=out)
+    if M:
+        e = _epilogue(out, N, bias, act, scale, residual)
+        _run(a.device, f"ea_gemm_fp8 M{M} N{N} K{a.cols}", _lib().ea_gemm_fp8, _p(a.q), _p(a.scale), _p(w.q), _p(w.scale), M, N, a.cols, C.byref(e))
+    return out
+
+
+def gemm_fp8_wgrad(dy, x):
+    """Gradients of a Linear's weight and bias from its 8-bit input: dy fp16 [..., N], x an Fp8Tensor of rows [..., K] (|values| <=
+    131008) -> (dw fp32 [N, K] = dy^T x, db fp32 [N]), both summed in fp32 in a fixed order."""
+    M, N = _rows_of("dy", dy, (torch.float16,))
+    _rows_fp8("x", x)
+    _need(x.rows == M, f"gemm_fp8_wgrad: dy has {M} rows, x {x.rows}")
+    K = x.cols
+    _check_fp8(dy.device, dy=dy, x=x.q, x_scale=x.scale)
+    if not M:
+        return torch.zeros((N, K), dtype=torch.float32, device=dy.device), torch.zeros((N,), dtype=torch.float32, device=dy.device)
+    lib = _lib()
+    dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
+    db = torch.empty((N,), dtype=torch.float32, device=dy.device)
+    nbytes = lib.ea_gemm_fp8_wgrad_workspace_bytes(M, N, K)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dy.device) if nbytes else None
+    _run(dy.device, f"ea_gemm_fp8_wgrad M{M} N{N} K{K}", lib.ea_gemm_fp8_wgrad, _p(dy), _p(x.q), _p(x.scale), _p(dw), _p(db), M, N, K, _p(ws), nbytes)
+    return dw, db

@@ -399,6 +399,43 @@ int ea_silu_f32(const float* x, float* out, long long n, void* stream);
 /* out = a + b (fp16), n % 8 == 0. */
 int ea_add_f16(const void* a, const void* b, void* out, long long n, void* stream);
 
+/* ---- Training operators on the 8-bit block format.  A row of C values is cut into blocks of 128 (the last padded with zero
+ * codes): e4m3 codes [rows][Kp], Kp = C rounded up to 128, and one exponent per block, stored as the byte E + 127 in
+ * scale[Kp / 128][Rp], Rp = rows rounded up to 16; a code stands for code * 2^E.  E is the smallest whole number in [-100, 120]
+ * with max |x| <= 448 * 2^E over the block's finite values (0 for zeros); non-finite values become NaN codes.  A weight has
+ * one exponent for 128 rows x 128 columns: scale[Kp / 128][ceil(rows / 128)].  Code pointers are 16-byte aligned, scales of rows 4.
+ * ea_quantize_fp8 / ea_quantize_fp8_weight: x / w fp16 (in_f32 = 0) or fp32, dense rows.
+ * ea_dequantize_fp8: block_rows = 1 (rows) or 128 (weight); out dense fp16 or fp32. */
+int ea_quantize_fp8(const void* x, int in_f32, void* q, unsigned char* scale, long long rows, int cols, void* stream);
+int ea_quantize_fp8_weight(const void* w, int in_f32, void* q, unsigned char* scale, int N, int K, void* stream);
+int ea_dequantize_fp8(const void* q, const unsigned char* scale, int block_rows, void* out, int out_f32, long long rows, int cols,
+                      void* stream);
+/* Activation that keeps its input in 8 bits.  act: EA_ACT_SILU, EA_ACT_GELU (z fp16 [M][H]) or EA_ACT_GEGLU (z fp16 [M][2 H] =
+ * [value | gate], h = value * gelu(gate)).  Output h fp16 [M][H], or hq / hscale in 8 bits (exactly one of h, hq).  zq / zscale: z as
+ * 8-bit rows of H (GEGLU: 2 M rows, a row's value and gate halves one after the other).
+ * ea_activation_fp8_bwd: dz = dh * act'(decoded z), fp16, z's layout. */
+int ea_activation_fp8(const void* z, int act, void* h, void* hq, unsigned char* hscale, void* zq, unsigned char* zscale, long long M, int H,
+                      void* stream);
+int ea_activation_fp8_bwd(const void* dh, const void* zq, const unsigned char* zscale, int act, void* dz, long long M, int H, void* stream);
+/* LayerNorm for training, C <= 4096.  Forward: y fp16 or q / scale in 8 bits (exactly one of y, q), stats fp32 [M][2] = (mean,
+ * 1 / sigma).  Backward: x_kind 0 fp16, 1 fp32, 2 8-bit (x_scale); residual (NULL: none) is added to dx and has its type (fp16, or
+ * fp32 where dx_f32); dgamma_dbeta fp32 [2][C].  The two column reductions have a fixed order. */
+int ea_layernorm_train(const void* x, int in_f32, const float* gamma, const float* beta, float eps, void* y, void* q, unsigned char* scale,
+                       float* stats, int M, int C, void* stream);
+size_t ea_layernorm_bwd_workspace_bytes(int M, int C);
+int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const unsigned char* x_scale, const float* stats, const float* gamma,
+                     const void* residual, void* dx, int dx_f32, float* dgamma_dbeta, int M, int C, void* workspace, size_t ws_bytes,
+                     void* stream);
+/* out = residual + scale * act(A W^T + bias): A 8-bit rows [M][Kp], W an 8-bit weight [N][Kp].  Of the epilogue: bias (per column), act
+ * (none, SiLU, GELU), scale, residual or residual32, out / out_f32, ldc, ldr; anything else is EA_ERR_UNSUPPORTED. */
+int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K,
+                const ea_epilogue* e, void* stream);
+/* Gradients of a Linear's weight and bias from its 8-bit input: dw fp32 [N][K] = dy^T x, db fp32 [N] = column sums of dy (fp16 [M][N]).
+ * Decoded inputs have to lie within +-131008.  The sums have a fixed order. */
+size_t ea_gemm_fp8_wgrad_workspace_bytes(int M, int N, int K);
+int ea_gemm_fp8_wgrad(const void* dy, const void* x, const unsigned char* x_scale, float* dw, float* db, int M, int N, int K, void* workspace,
+                      size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,6 +2,8 @@
 // ea_gemm_fp8_wgrad, the weight and bias gradient of a Linear from its 8-bit input.
 #include "ea_fp8_gemm.h"
 
+int ea_forced_variant();          // ea_gemm.hip: the calling thread's ea_tuning.variant (tests)
+
 namespace {
 
 // ---------------------------------------------------------------------------------------------------- weight gradient
@@ -164,16 +166,44 @@ int wgrad_splits(int M, int N, int K) {
   return s < 1 ? 1 : s;
 }
 
+long long fp8_tiles(const EaFp8GemmParams& p, int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); }
+
 template <int BM, int BN, int WM, int WN, int S>
-int fp8_ring_launch(EaFp8GemmParams& p, void* stream) {
+int fp8_ring_launch(const EaFp8GemmParams& p, void* stream) {
   auto k = ea_fp8_ring_kernel<BM, BN, WM, WN, S>;
-  const int smem = (BM + BN) * 128 * S;
-  const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  const int smem = (BM + BN) * 128 * S + EA_F8_CH * (BM + 4);
+  const long long tiles = fp8_tiles(p, BM, BN);
   if (tiles > 0x7fffffffll) return EA_ERR_BAD_SHAPE;
-  p.raster_gm = 8;
   ea_allow_big_lds(k, smem);
   EA_LAUNCH(k, dim3((unsigned)tiles), dim3(64 * WM * WN), smem, stream, p);
   return ea_launch_status();
+}
+int fp8_large_launch(const EaFp8GemmParams& p, void* stream) {
+  const long long tiles = fp8_tiles(p, 256, 256);
+  if (tiles > 0x7fffffffll) return EA_ERR_BAD_SHAPE;
+  auto k = ea_fp8_large_kernel;
+  ea_allow_big_lds(k, EA_F8L_LDS);
+  EA_LAUNCH(k, dim3((unsigned)tiles), dim3(512), EA_F8L_LDS, stream, p);
+  return ea_launch_status();
+}
+
+// Which kernel (times in us on the MI355X, M x N x K):
+//   256 x 256 tiles, one workgroup per CU: from 8 K tiles on, where the last round of 256 workgroups is at least as full as three
+//       quarters of all rounds.  16384 x 5120 x 1280 115 (128 x 128: 126), 8192^3 391 (504); 16384 x 1280 x 5120 fills 1.25 rounds:
+//       123 (115), and 5 K tiles do not carry the larger tile's start and end: 8192 x 5120 x 640 62 (57)
+//   128 x 128, two workgroups per CU (one multiplies while the other starts or stores): from 256 tiles on.  32768 x 320 x 320 17.0
+//       (64 x 128: 16.1, 64 x 64: 22.7), 16384 x 5120 x 1280 126 (154, 231)
+//   64 x 128: from 160 tiles on.  616 x 2560 x 1024 6.6 (64 x 64: 7.3, 128 x 128: 8.5), 2048 x 1280 x 1280 9.9 (12.9, 9.9)
+//   64 x 64 with a ring of four: few tiles, where each K tile's latency counts.  512 x 1280 x 5120 15.8 (64 x 128: 24.1),
+//       77 x 1024 x 1024 5.7 (5.9)
+int fp8_launch(EaFp8GemmParams& p, void* stream) {
+  p.raster_gm = 8;                         // (4 and 16: within 2 %)
+  const int v = ea_forced_variant();
+  const long long large = fp8_tiles(p, 256, 256), rounds = (large + 255) / 256;
+  if (v == 101 || (v < 101 && p.nb >= 8 && large * 4 >= rounds * 256 * 3)) return fp8_large_launch(p, stream);
+  if (v == 102 || (v < 101 && fp8_tiles(p, 128, 128) >= 256)) return fp8_ring_launch<128, 128, 2, 4, 2>(p, stream);
+  if (v == 103 || (v < 101 && fp8_tiles(p, 64, 128) >= 160)) return fp8_ring_launch<64, 128, 2, 4, 2>(p, stream);
+  return fp8_ring_launch<64, 64, 2, 2, 4>(p, stream);
 }
 
 }  // namespace
@@ -193,9 +223,11 @@ extern "C" int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const vo
   p.M = M; p.N = N; p.nb = ea_fp8_blocks(K); p.Kp = p.nb * EA_FP8_BLOCK; p.nwb = (N + 127) / 128; p.Rp = ea_fp8_scale_pitch(M);
   p.bias = e->bias; p.residual = (const f16*)e->residual; p.residual32 = e->residual32; p.out = e->out;
   p.act = e->act; p.out_f32 = e->out_f32; p.ldc = e->ldc; p.ldr = e->ldr; p.scale = e->scale;
-  p.vec = (N & 7) == 0 && (e->ldc & 7) == 0 && ((uintptr_t)e->out & 15) == 0 &&
-          ((!e->residual && !e->residual32) || ((e->ldr & 7) == 0 && ((((uintptr_t)e->residual) | ((uintptr_t)e->residual32)) & 15) == 0));
-  return fp8_ring_launch<128, 128, 2, 2, 2>(p, stream);
+  // 16-byte accesses; a tile's 256 rows within 2 GiB
+  p.vec = (N & 7) == 0 && (e->ldc & 7) == 0 && e->ldc < (1 << 21) && ((uintptr_t)e->out & 15) == 0;
+  if (e->residual || e->residual32)
+    p.vec = p.vec && (e->ldr & 7) == 0 && e->ldr < (1 << 21) && ((((uintptr_t)e->residual) | ((uintptr_t)e->residual32)) & 15) == 0;
+  return fp8_launch(p, stream);
 }
 
 extern "C" size_t ea_gemm_fp8_wgrad_workspace_bytes(int M, int N, int K) {

@@ -840,6 +840,8 @@ static int launch_pair(EaGemmParams& p, EaGemmParams& q, void* workspace, size_t
 
 }  // namespace
 
+int ea_forced_variant() { return g_tune.variant; }
+
 extern "C" int ea_set_tuning(const ea_tuning* t) {
   if (t) g_tune = *t;
   else g_tune = ea_tuning{0, 0, 0, 0, 0, 0};

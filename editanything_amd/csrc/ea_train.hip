@@ -275,11 +275,11 @@ __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
   }
 }
 
-// out[c] = sum_g part[g][c] in a fixed order: a workgroup owns 32 columns, 32 lanes of partials each
-__global__ __launch_bounds__(1024) void ea_ln_join_kernel(const float* part, float* out, int G, int cols) {
+// dgamma | dbeta [c] = sum_g part[g][c] in a fixed order: a workgroup owns 32 columns, 32 lanes of partials each
+__global__ __launch_bounds__(1024) void ea_ln_join_kernel(const float* part, float* dgamma, float* dbeta, int G, int C) {
   EA_SMEM(smem);
   float* red = reinterpret_cast<float*>(smem);      // [32][33]
-  const int cx = threadIdx.x & 31, gy = threadIdx.x >> 5;
+  const int cx = threadIdx.x & 31, gy = threadIdx.x >> 5, cols = 2 * C;
   const int c = blockIdx.x * 32 + cx;
   float s = 0.0f;
   if (c < cols)
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(1024) void ea_ln_join_kernel(const float* part, flo
     if (gy < h) red[gy * 33 + cx] += red[(gy + h) * 33 + cx];
     __syncthreads();
   }
-  if (gy == 0 && c < cols) out[c] = red[cx];
+  if (gy == 0 && c < cols) (c < C ? dgamma[c] : dbeta[c - C]) = red[cx];
 }
 
 bool ln_vec(int C, const void* a, const void* b, const void* c, const void* d, const void* e, const void* f) {
@@ -363,9 +363,9 @@ extern "C" size_t ea_layernorm_bwd_workspace_bytes(int M, int C) {
 }
 
 extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const unsigned char* x_scale, const float* stats,
-                                const float* gamma, const void* residual, void* dx, int dx_f32, float* dgamma_dbeta, int M, int C,
+                                const float* gamma, const void* residual, void* dx, int dx_f32, float* dgamma, float* dbeta, int M, int C,
                                 void* workspace, size_t ws_bytes, void* stream) {
-  if (!dy || !x || !stats || !gamma || !dx || !dgamma_dbeta || !workspace || (x_kind == XK_FP8 && !x_scale)) return EA_ERR_BAD_ARG;
+  if (!dy || !x || !stats || !gamma || !dx || !dgamma || !dbeta || !workspace || (x_kind == XK_FP8 && !x_scale)) return EA_ERR_BAD_ARG;
   if (x_kind < XK_F16 || x_kind > XK_FP8) return EA_ERR_BAD_ARG;
   if (M <= 0 || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)stats & 7) || ((uintptr_t)workspace & 3)) return EA_ERR_BAD_ARG;
@@ -381,6 +381,6 @@ extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const
                                   : ln_bwd_launch<XK_FP8>(p, vec, grid, stream);
   if (st != EA_OK) return st;
   auto k = ea_ln_join_kernel;
-  EA_LAUNCH(k, dim3((2 * C + 31) / 32), dim3(1024), 32 * 33 * sizeof(float), stream, (const float*)workspace, dgamma_dbeta, grid, 2 * C);
+  EA_LAUNCH(k, dim3((2 * C + 31) / 32), dim3(1024), 32 * 33 * sizeof(float), stream, (const float*)workspace, dgamma, dbeta, grid, C);
   return ea_launch_status();
 }

@@ -142,7 +142,8 @@ typedef struct ea_tuning {
   int32_t force_generic;       /* 1: the register-staged generic kernel for everything */
   int32_t variant;             /* 0 auto, k: force instantiation k of the LDS-DMA kernels (1 / 9: ea_gemm2.h 128- / 64-row tiles,
                                   30: ea_gemm8.h 256 x 256 tiles, 33 / 34: the 64- / 128-row tiles with a 3-stage ring -- two K tiles in flight, for
-                                  weights that come from HBM; the rest: tools builds) */
+                                  weights that come from HBM; 101 ... 104: ea_gemm_fp8's 256 x 256, 128 x 128, 64 x 128 and
+                                  64 x 64 tiles; the rest: tools builds) */
   int32_t splits;              /* 0 plan's own, s: force the split-K factor */
   int32_t bn;                  /* 0 plan's own, 128: force 128-wide column tiles */
   int32_t no_register_direct;  /* 1: LDS-slab epilogue where the register-direct one would run */
@@ -419,13 +420,13 @@ int ea_activation_fp8(const void* z, int act, void* h, void* hq, unsigned char* 
 int ea_activation_fp8_bwd(const void* dh, const void* zq, const unsigned char* zscale, int act, void* dz, long long M, int H, void* stream);
 /* LayerNorm for training, C <= 4096.  Forward: y fp16 or q / scale in 8 bits (exactly one of y, q), stats fp32 [M][2] = (mean,
  * 1 / sigma).  Backward: x_kind 0 fp16, 1 fp32, 2 8-bit (x_scale); residual (NULL: none) is added to dx and has its type (fp16, or
- * fp32 where dx_f32); dgamma_dbeta fp32 [2][C].  The two column reductions have a fixed order. */
+ * fp32 where dx_f32); dgamma, dbeta fp32 [C], reduced in a fixed order. */
 int ea_layernorm_train(const void* x, int in_f32, const float* gamma, const float* beta, float eps, void* y, void* q, unsigned char* scale,
                        float* stats, int M, int C, void* stream);
 size_t ea_layernorm_bwd_workspace_bytes(int M, int C);
 int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const unsigned char* x_scale, const float* stats, const float* gamma,
-                     const void* residual, void* dx, int dx_f32, float* dgamma_dbeta, int M, int C, void* workspace, size_t ws_bytes,
-                     void* stream);
+                     const void* residual, void* dx, int dx_f32, float* dgamma, float* dbeta, int M, int C, void* workspace,
+                     size_t ws_bytes, void* stream);
 /* out = residual + scale * act(A W^T + bias): A 8-bit rows [M][Kp], W an 8-bit weight [N][Kp].  Of the epilogue: bias (per column), act
  * (none, SiLU, GELU), scale, residual or residual32, out / out_f32, ldc, ldr; anything else is EA_ERR_UNSUPPORTED. */
 int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K,

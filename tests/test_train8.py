@@ -337,9 +337,9 @@ def test_layernorm_backward(kb, M, C, kind, res):
         q, e = quantize(x)
         x, xs, x64 = q, pack_scales(e), values(q, e, C)
     st = np.stack([mu, r], 1).astype(np.float32)
-    dx, dgb = kb.up(np.full((M + 1, C), 7, out)), kb.zeros((2, C), np.float32)
+    dx, dg, db = kb.up(np.full((M + 1, C), 7, out)), kb.zeros((C,), np.float32), kb.zeros((C,), np.float32)
     ws = kb.zeros((kb.lib.ea_layernorm_bwd_workspace_bytes(M, C) // 4,), np.float32)
-    args = (ptr(dy), ptr(x), kind, ptr(xs), ptr(st), ptr(gamma), ptr(residual), ptr(dx), int(kind == 1), ptr(dgb), M, C, ptr(ws))
+    args = (ptr(dy), ptr(x), kind, ptr(xs), ptr(st), ptr(gamma), ptr(residual), ptr(dx), int(kind == 1), ptr(dg), ptr(db), M, C, ptr(ws))
     assert kb.lib.ea_layernorm_bwd(*args, ws.nbytes - 1 if kb.name == "emu" else ws.numel() * 4 - 1, kb.stream) == -4
     assert kb.lib.ea_layernorm_bwd(*args, ws.nbytes if kb.name == "emu" else ws.numel() * 4, kb.stream) == 0
     mu, r = st.astype(np.float64).T
@@ -358,7 +358,7 @@ def test_layernorm_backward(kb, M, C, kind, res):
     assert np.isinf(got[:M][over]).all()
     err = np.abs(np.where(over, 0, got[:M]) - np.where(over, 0, ref))
     assert (err <= (U32 if kind == 1 else U16) * np.abs(ref) + (0 if kind == 1 else TINY16) + 1.01 * tol + 4 * U32 * np.abs(ref)).all()
-    dg, db = kb.down(dgb).astype(np.float64)
+    dg, db = kb.down(dg).astype(np.float64), kb.down(db).astype(np.float64)
     assert (np.abs(dg - (d * n).sum(0)) <= (M + 4) * U32 * np.abs(d * n).sum(0) + (np.abs(d) * nerr).sum(0) + 1e-30).all()
     assert (np.abs(db - d.sum(0)) <= (M + 2) * U32 * np.abs(d).sum(0)).all()
 
@@ -399,6 +399,14 @@ def gemm_case(M, N, K, seed=12):
     return aq, pack_scales(ae), wq, (we + 127).astype(np.uint8), a @ w.T, np.abs(a) @ np.abs(w).T
 
 
+def force(kb, kernel):
+    """Pin one of gemm_fp8's kernels (0: the launch rule's own choice)."""
+    if kernel:
+        assert L.set_tuning(kb.lib, variant=kernel) == 0
+
+
+KERNELS = [0, 101, 102, 103, 104]
+
 # The matrix unit adds 8 neighbouring products of 8-bit operands before they meet the fp32 accumulator, each product cut towards zero at
 # 2^-13 of the power of two of the eight's largest (measured: beside 256, seven products of 256 * 2^-13 all count and seven of
 # 256 * 2^-14 all vanish, whatever their sign; products of other eights and the accumulator lose nothing).  So an eight is off by at
@@ -408,9 +416,13 @@ UNIT = 7 * 2.0 ** -13
 GEMM_SHAPES = [(1, 1, 1), (1, 128, 128), (16, 8, 130), (70, 100, 300), (128, 256, 256), (130, 72, 640), (33, 7, 77), (200, 264, 200)]
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("form", ["plain", "bias gelu fp32", "bias silu residual", "residual32 scale"])
 @pytest.mark.parametrize("M,N,K", GEMM_SHAPES)
-def test_gemm_fp8(kb, M, N, K, form):
+def test_gemm_fp8(kb, M, N, K, form, kernel):
+    if kb.name == "emu" and kernel and (M, N) not in ((1, 1), (70, 100), (130, 72)):
+        pytest.skip("every kernel at three shapes on the emulation, at all of them on the GPU")
+    force(kb, kernel)
     aq, sa, wq, sw, ref, mag = gemm_case(M, N, K)
     g = np.random.default_rng(13)
     f32out = "fp32" in form
@@ -433,8 +445,9 @@ def test_gemm_fp8(kb, M, N, K, form):
     assert (np.abs(got[:M] - v) <= scale * err + (2 * U32 if f32out else U16) * np.abs(v) + TINY16 + 4 * U32 * np.abs(v)).all()
 
 
-@pytest.mark.parametrize("M,N,K", GEMM_SHAPES + [(300, 520, 512), (257, 300, 1300)])
-def test_gemm_fp8_whole_numbers_exactly(kb, M, N, K):
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("M,N,K", GEMM_SHAPES + [(300, 520, 512), (257, 300, 1300), (17, 24, 8450)])
+def test_gemm_fp8_whole_numbers_exactly(kb, M, N, K, kernel):
     """Whole numbers up to 8 under per-block powers of two: every product and sum is a whole number of small steps that fp32 and the
     matrix unit hold, so the result has to be exact -- each row, column, block and scale in its place."""
     g = np.random.default_rng(19)
@@ -444,6 +457,7 @@ def test_gemm_fp8_whole_numbers_exactly(kb, M, N, K):
     ea, ew = g.integers(-2, 3, (nb, M)), g.integers(-1, 2, (nb, -(-N // 128)))
     aq, wq = encode(a), encode(w)
     out = kb.up(np.full((M + 1, N), 7, np.float32))
+    force(kb, kernel)
     assert kb.lib.ea_gemm_fp8(ptr(aq), ptr(pack_scales(ea)), ptr(wq), ptr((ew + 127).astype(np.uint8)), M, N, K, ctypes.byref(epilogue(out)),
                               kb.stream) == 0
     ref = values(aq, ea, K) @ (decode(wq) * np.repeat(np.repeat(2.0 ** ew.T, 128, 0)[:N], 128, 1))[:, :K].T
@@ -536,10 +550,10 @@ def test_the_c_entries_refuse(emu_lib):
     assert lib.ea_layernorm_train(p, 0, p, p, 1e-5, None, None, None, p, 1, 8, None) == -2
     assert lib.ea_layernorm_train(p, 0, p, p, 1e-5, o, None, None, p, 1, 4097, None) == -1
     assert lib.ea_layernorm_train(p, 0, p, p, 1e-5, o, None, None, p + 4, 1, 8, None) == -2
-    assert lib.ea_layernorm_bwd(p, p, 3, None, p, p, None, o, 0, o, 1, 8, p, 1 << 20, None) == -2
-    assert lib.ea_layernorm_bwd(p, p, 2, None, p, p, None, o, 0, o, 1, 8, p, 1 << 20, None) == -2
-    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, 0, o, 1, 5000, p, 1 << 20, None) == -1
-    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, 0, o, 1, 8, p, 0, None) == -4
+    assert lib.ea_layernorm_bwd(p, p, 3, None, p, p, None, o, 0, o, o, 1, 8, p, 1 << 20, None) == -2
+    assert lib.ea_layernorm_bwd(p, p, 2, None, p, p, None, o, 0, o, o, 1, 8, p, 1 << 20, None) == -2
+    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, 0, o, o, 1, 5000, p, 1 << 20, None) == -1
+    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, 0, o, o, 1, 8, p, 0, None) == -4
     assert lib.ea_layernorm_bwd_workspace_bytes(0, 8) == 0 and lib.ea_layernorm_bwd_workspace_bytes(1, 4097) == 0
     e = epilogue(a)
     g = lambda **kw: lib.ea_gemm_fp8(kw.get("a", p), kw.get("sa", p), p, p, kw.get("M", 16), kw.get("N", 16), kw.get("K", 128),  # noqa: E731

@@ -11,11 +11,12 @@ namespace {
 // The sum runs over rows, and each row has its own exponents, so the matrix unit's block scales do not apply (they belong to runs of
 // the contracted axis).  x is decoded to fp16 instead -- four significant bits, exact -- and multiplied by dy as it is: every product
 // is exact, the sums are fp32.  x is decoded as x / 2 and the accumulators are doubled: e4m3 rounding can carry an fp16 maximum
-// (65504) to 65536, and at the small end x / 2 loses less than fp16's own last step.  Values beyond +-131008 become infinite.
-//
-// Both operands have the contracted axis as their ROW axis.  Tiles go to LDS row-major and the fragments are read transposed
-// (ds_read_b64_tr_b16): 16 lanes take a 4 x 16 block and each ends up with 4 consecutive rows of one column.  A wave reads 16 rows of
-// 32 bytes at once; 32-byte pieces are XORed with the row so that these cover all 64 banks twice, the minimum.
+// (65504) to 65536, and at the small end x / 2 loses no more than fp16's own last step.  Blocks whose maximum exceeds 448 * 2^8 = 114688
+// become infinite.
+// Both operands have the contracted axis as their ROW axis, so they go to LDS row-major and the fragments are read transposed: 16 lanes
+// take a 4 x 16 (fp16) or 8 x 16 (codes) block and each ends up with consecutive rows of one column.  Bound by the matrix unit at
+// the fp16 rate: 8192^3 915 us = 1200 TFLOP/s (the library's fp16 product: 1382).
+// First the kernel for any N and alignment: 128 x 128 tiles, both operands through registers, x decoded on the way to LDS.
 struct WgradParams {
   const f16* dy; const uint8_t* x; const uint8_t* sx;
   float* dw; float* db;              // or one [N][K] + [N] partial per slice
@@ -28,12 +29,21 @@ constexpr int WG_BUF = WG_R * WG_T * 2;                  // one operand's tile: 
 // byte of (row, column) in a tile
 __device__ __forceinline__ int wg_at(int r, int c) { return r * 256 + ((((c >> 4) ^ r) & 7) << 5) + (c & 15) * 2; }
 
+// 4 rows of one column of fp16 (the builtin, not ea_prims.h's inline assembly: the compiler then knows when the registers are written)
+__device__ __forceinline__ f16x4 wg_read_tr16(const char* ptr) {
+#ifdef EA_EMU
+  return ea_lds_read_tr16<0>(ptr);
+#else
+  typedef __fp16 h4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4*)ptr));
+#endif
+}
 __device__ __forceinline__ f16x8 wg_frag(const char* buf, int r0, int c0, int lane) {
   const int q = lane >> 4, i = lane & 15;
   // rows r0 + 4 q .. + 3 and r0 + 16 + 4 q .. + 3: the order of rows inside a step is the same for both operands
   const char* a = buf + wg_at(r0 + 4 * q + (i >> 2), c0 + (i & 3) * 4);
   const char* b = buf + wg_at(r0 + 16 + 4 * q + (i >> 2), c0 + (i & 3) * 4);
-  const f16x4 lo = ea_lds_read_tr16<0>(a), hi = ea_lds_read_tr16<0>(b);
+  const f16x4 lo = wg_read_tr16(a), hi = wg_read_tr16(b);
   return f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
@@ -43,6 +53,17 @@ __device__ __forceinline__ void wg_decode16(u32x4 w, float s, f16x8& a, f16x8& b
   for (int i = 0; i < 4; ++i) ea_fp8_unpack4(w[i], v + 4 * i);
 #pragma unroll
   for (int j = 0; j < 8; ++j) { a[j] = (f16)(v[j] * s); b[j] = (f16)(v[8 + j] * s); }
+}
+
+// doubled accumulators to row[k ... k + 3]
+__device__ __forceinline__ void wg_store4(float* row, int k, int K, f32x4 v) {
+  if ((K & 3) == 0) {
+    if (k < K) *reinterpret_cast<f32x4*>(row + k) = v * 2.0f;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (k + r < K) row[k + r] = v[r] * 2.0f;
+  }
 }
 
 __global__ __launch_bounds__(256) void ea_fp8_wgrad_kernel(WgradParams p) {
@@ -116,54 +137,495 @@ __global__ __launch_bounds__(256) void ea_fp8_wgrad_kernel(WgradParams p) {
       for (int i = 0; i < 4; ++i) fd[i] = wg_frag(smem, h, wn * 64 + i * 16, lane);
 #pragma unroll
       for (int j = 0; j < 4; ++j) fx[j] = wg_frag(smem + WG_BUF, h, wk * 64 + j * 16, lane);
-      ea_lds_tr_wait();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = ea_mfma_16x16x32(fd[i], fx[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) acc[i][j] = ea_mfma_16x16x32(fx[j], fd[i], acc[i][j]);
       if (tk == 0 && wk == 0)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) accb[i] = ea_mfma_16x16x32(fd[i], ones, accb[i]);
+        for (int i = 0; i < 4; ++i) accb[i] = ea_mfma_16x16x32(ones, fd[i], accb[i]);
     }
   }
   float* dw = p.dw + (long long)blockIdx.y * p.part;
   float* db = p.splits > 1 ? dw + (long long)p.N * p.K : p.db;
   const int l15 = lane & 15, lq = lane >> 4;
 #pragma unroll
+  for (int i = 0; i < 4; ++i) {            // D^T: a lane holds 4 consecutive k of one n
+    const int n = n0 + wn * 64 + i * 16 + l15;
+    if (n >= p.N) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wk * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
+    if (tk == 0 && wk == 0 && lq == 0) db[n] = accb[i][0];
+  }
+}
+
+// -------------------------------------------------------------------------------------------- weight gradient, large tiles
+// 256 n x 256 k, 8 waves (2 x 4) of 128 x 64, 64 rows per step, two steps of LDS, in the manner of ea_fp8_gemm.h's large kernel: four
+// phases of one 64 x 32 quadrant (16 MFMAs), each a load part and a multiply part with a barrier behind either, the two wave rows one
+// barrier apart, so that on every SIMD one wave multiplies while the other reads, decodes and issues DMA.
+// Both operands go to LDS as they are.  dy: half h holds the 64-column quadrants h of both wave rows, rows of 256 bytes, read with
+// ds_read_b64_tr_b16; x: half h holds the 32-column quadrants h of the four wave columns, rows of 128 bytes of CODES, read with
+// ds_read_b64_tr_b8: 16 lanes take 8 rows x 16 bytes and each gets 8 rows of one column.  The codes become fp16 in registers,
+//     x / 2 = (code 2^-8) * 2^(E + 7):   the conversion's own scale does the first factor, a packed fp16 product with the rows' 8 scale
+// factors (one 16-byte LDS read for 8 rows) the second; both are exact while x / 2 is an fp16 value.  E above 8 gives infinities, E below
+// -31 (|x| < 2^-23) zeros.
+// The load parts: L0 reads dy quadrant 0, L1 reads and decodes x quadrant 1, L2 reads dy quadrant 1, L3 reads and decodes the next
+// step's x quadrant 0 (1.58 us per step with the chip two fifths full; decoding in the multiply parts
+// 1.71, spreading the dy reads over all four load parts 1.61).  DMA of the next step: x in L0, dy 0 in L1,
+// dy 1 in L2.  What L(q) issues is waited for in L(q + 2) (counted: the younger two parts' DMA stays in flight) and first read in
+// L(q + 3), one barrier after the lagging wave row's wait.
+constexpr int WL_DY = 32768, WL_X = 16384, WL_STEP = WL_DY + WL_X, WL_CH = 32;      // bytes per step; steps whose scale factors are in LDS
+constexpr int WL_SCL = 2 * WL_STEP, WL_LDS = WL_SCL + WL_CH * 2 * 64 * 2;
+
+// 32-byte piece of a dy row, 16-byte piece of an x row: XORed so that the rows that a wave reads together cover the banks evenly
+__device__ __forceinline__ int wl_dy_swz(int r) { return (r & 3) | ((r >> 1) & 4); }
+__device__ __forceinline__ int wl_x_swz(int r) { return (r >> 1) & 7; }
+
+#ifdef EA_EMU
+// ds_read_b64_tr_b8: 16 lanes take 8 rows x 16 bytes (lanes 2 r, 2 r + 1: row r); lane i gets column i
+inline u32x2 wl_emu_tr8(const char* ptr) {
+  char* sc = ea_emu::wave_scratch();
+  const int l = ea_emu::lane_id(), g = l & ~15, i = l & 15;
+  memcpy(sc + l * 64, ptr, 8);
+  ea_emu::wave_sync();
+  uint8_t b[8];
+  for (int r = 0; r < 8; ++r) b[r] = (uint8_t)sc[(g + 2 * r + (i >> 3)) * 64 + (i & 7)];
+  ea_emu::wave_sync();
+  u32x2 v;
+  memcpy(&v, b, 8);
+  return v;
+}
+#endif
+// The fragment reads of one phase.  Inline assembly, because the compiler waits for all LDS-DMA in front of a transposed read that it
+// knows (its address may be the one being filled); with the wait for the reads in the same block, no register is in flight behind it.
+// Fragment i: rows 8 lq ... + 7 of both 32-row halves.
+template <int Q>
+__device__ __forceinline__ void wl_read_d(const char* a0, const char* a1, const char* a2, const char* a3, f16x8 (&f)[4][2]) {
+  const char* const ptr[4] = {a0, a1, a2, a3};
+#ifdef EA_EMU
+  for (int i = 0; i < 4; ++i)
+    for (int ks = 0; ks < 2; ++ks) {
+      const f16x4 lo = ea_lds_read_tr16<0>(ptr[i] + Q + ks * 8192), hi = ea_lds_read_tr16<0>(ptr[i] + Q + ks * 8192 + 1024);
+      f[i][ks] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+#else
+  unsigned ad[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ad[i] = (unsigned)(uintptr_t)ptr[i];
+  f16x4 r[4][4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16 offset:%20\n\tds_read_b64_tr_b16 %1, %16 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %2, %16 offset:%22\n\tds_read_b64_tr_b16 %3, %16 offset:%23\n\t"
+      "ds_read_b64_tr_b16 %4, %17 offset:%20\n\tds_read_b64_tr_b16 %5, %17 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %6, %17 offset:%22\n\tds_read_b64_tr_b16 %7, %17 offset:%23\n\t"
+      "ds_read_b64_tr_b16 %8, %18 offset:%20\n\tds_read_b64_tr_b16 %9, %18 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %10, %18 offset:%22\n\tds_read_b64_tr_b16 %11, %18 offset:%23\n\t"
+      "ds_read_b64_tr_b16 %12, %19 offset:%20\n\tds_read_b64_tr_b16 %13, %19 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %14, %19 offset:%22\n\tds_read_b64_tr_b16 %15, %19 offset:%23\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3]),
+        "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[2][2]), "=&v"(r[2][3]), "=&v"(r[3][0]), "=&v"(r[3][1]), "=&v"(r[3][2]), "=&v"(r[3][3])
+      : "v"(ad[0]), "v"(ad[1]), "v"(ad[2]), "v"(ad[3]), "n"(Q), "n"(Q + 1024), "n"(Q + 8192), "n"(Q + 9216)
+      : "memory");
+#pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = n0 + wn * 64 + i * 16 + 4 * lq + r;
-      if (n >= p.N) continue;
+    for (int ks = 0; ks < 2; ++ks)
+      f[i][ks] = __builtin_shufflevector(r[i][2 * ks], r[i][2 * ks + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+#endif
+}
+template <int Q>
+__device__ __forceinline__ void wl_read_x(const char* a0, const char* a1, u32x2 (&f)[2][2]) {
+#ifdef EA_EMU
+  for (int j = 0; j < 2; ++j)
+    for (int ks = 0; ks < 2; ++ks) f[j][ks] = wl_emu_tr8((j ? a1 : a0) + Q + ks * 4096);
+#else
+  asm volatile("ds_read_b64_tr_b8 %0, %4 offset:%6\n\tds_read_b64_tr_b8 %1, %4 offset:%7\n\t"
+               "ds_read_b64_tr_b8 %2, %5 offset:%6\n\tds_read_b64_tr_b8 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1])
+               : "v"((unsigned)(uintptr_t)a0), "v"((unsigned)(uintptr_t)a1), "n"(Q), "n"(Q + 4096)
+               : "memory");
+#endif
+}
+// LDS-DMA through a descriptor with an end: what lies behind it arrives as zeros
+__device__ __forceinline__ void wl_dma16(ea_rows r, unsigned off, char* lds_base) {
+#ifdef EA_EMU
+  const u32x4 v = ea_rows_load(r, off);
+  memcpy(lds_base + 16 * ea_emu::lane_id(), &v, 16);
+#else
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds_base, 16, off, 0, 0, 0);
+#endif
+}
+// 8 codes times their rows' factors
+__device__ __forceinline__ f16x8 wl_decode8(u32x2 w, f16x8 s) {
+#ifdef EA_EMU
+  f16x8 o;
+  for (int j = 0; j < 8; ++j) o[j] = (f16)((float)(f16)(ea_emu_fp8_to_f32((w[j >> 2] >> (8 * (j & 3))) & 255) * 0.00390625f) * (float)s[j]);
+  return o;
+#else
+  const u32x4 h = {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 0.00390625f, false)),
+                   __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 0.00390625f, true)),
+                   __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], 0.00390625f, false)),
+                   __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], 0.00390625f, true))};
+  return __builtin_bit_cast(f16x8, h) * s;
+#endif
+}
+// 2^(E + 7) as fp16 from the stored byte E + 127
+__device__ __forceinline__ f16 wl_factor(int byte) {
+  const int e = byte - 120;
+  const unsigned short u = e >= 16 ? 0x7c00 : e >= -14 ? (unsigned short)((e + 15) << 10) : e >= -24 ? (unsigned short)(1 << (e + 24)) : 0;
+  return __builtin_bit_cast(f16, u);
+}
+
+// an MFMA operand whose row q is ones: row q of the product is then the column sums of the other operand
+__device__ __forceinline__ f16x8 wl_unit_row(int q, int l15) {
+  unsigned u = l15 == q ? 0x3c003c00u : 0u;
+#ifndef EA_EMU
+  asm volatile("" : "+v"(u));              // (made where it is used: kept over the loop, its four registers were spilled)
+#endif
+  return __builtin_bit_cast(f16x8, u32x4{u, u, u, u});
+}
+
+// ------------------------------------------------------------------------------------- weight gradient, 128 x 128 tiles
+// Few or small outputs: 4 waves (2 x 2) of 64 x 64, a ring of three 64-row steps (24 KiB each, two workgroups per CU), one barrier per
+// step; operands, fragment reads and decoding as in the large kernel.
+constexpr int WR_S = 3, WR_DY = 16384, WR_STEP = 24576, WR_CH = 32, WR_SCL = WR_S * WR_STEP, WR_LDS = WR_SCL + WR_CH * 64 * 2;
+__global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p) {
+  EA_SMEM(smem);
+  const int tid = threadIdx.x, lane = tid & 63, wave = ea_uniform(tid >> 6), wm = wave >> 1, wn = wave & 1;
+  const int l15 = lane & 15, lq = lane >> 4;
+  const int tn = ea_uniform((int)blockIdx.x / p.tiles_k), tk = ea_uniform((int)blockIdx.x - tn * p.tiles_k);
+  const int n0 = tn * 128, k0 = tk * 128;
+  const int m_begin = blockIdx.y * p.rows_per_split;
+  const int m_end = m_begin + p.rows_per_split < p.M ? m_begin + p.rows_per_split : p.M;
+  const int steps = (m_end - m_begin + 63) >> 6;
+  unsigned vd[4], vx[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = k0 + wk * 64 + j * 16 + l15;
-        if (k < p.K) dw[(long long)n * p.K + k] = acc[i][j][r] * 2.0f;
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * (4 * wave + i) + (lane >> 4), c = ((((lane & 15) >> 1) ^ wl_dy_swz(r)) * 16) + (lane & 1) * 8;
+    vd[i] = n0 + c < p.N ? ((unsigned)r * (unsigned)p.N + (unsigned)c) * 2u : EA_F8_NOWHERE;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 8 * (2 * wave + i) + (lane >> 3);
+    vx[i] = (unsigned)r * (unsigned)p.Kp + (unsigned)(((lane & 7) ^ wl_x_swz(r)) * 16);
+  }
+  ea_rows rd = ea_make_rows(p.dy, 0), rx = ea_make_rows(p.x, 0);
+  auto stage = [&](int t) {                // t: step of the chunk
+    char* buf = smem + (t % WR_S) * WR_STEP;
+    const unsigned od = ea_uniform((unsigned)t * 64u * (unsigned)p.N * 2u), ox = ea_uniform((unsigned)t * 64u * (unsigned)p.Kp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wl_dma16(rd, vd[i] + od, buf + (4 * wave + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wl_dma16(rx, vx[i] + ox, buf + WR_DY + (2 * wave + i) * 1024);
+  };
+  int ad[4], ax[4];                        // fragment i is the wave's 16-column group i ^ 2 wn: it sums dy over the groups of fragments 0 and 1
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * lq + (l15 >> 2), s = 8 * lq + (l15 >> 1);
+    ad[i] = r * 256 + (((wm * 4 + (i ^ (2 * wn))) ^ wl_dy_swz(r)) << 5) + (l15 & 3) * 8;
+    ax[i] = WR_DY + s * 128 + (((wn * 4 + i) ^ wl_x_swz(s)) << 4) + (l15 & 1) * 8;
+  }
+  f32x4 acc[4][4], accb = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const bool sums = tk == 0;
+  char* const scl = smem + WR_SCL;
+  for (int t0 = 0; t0 < steps; t0 += WR_CH) {
+    const int n = steps - t0 < WR_CH ? steps - t0 : WR_CH;
+    const long long mc = m_begin + t0 * 64ll;
+    if (t0) ea_raw_barrier();              // the chunk before this one has been read
+    const int left = (int)(m_end - mc);
+    const uint8_t* const sx = p.sx + tk * p.Rp + mc;
+    unsigned char sb[WR_CH * 64 / 256];
+#pragma unroll
+    for (int u = 0; u < WR_CH * 64 / 256; ++u) sb[u] = u * 256 + tid < left ? sx[u * 256 + tid] : 0;      // (a row that is not there: factor 0)
+    rd = ea_make_rows(p.dy + mc * p.N + n0, ((m_end - mc) * p.N - n0) * 2);
+    rx = ea_make_rows(p.x + mc * p.Kp + k0, (m_end - mc) * p.Kp - k0);
+#pragma unroll
+    for (int t = 0; t < WR_S - 1; ++t)
+      if (t < n) stage(t);
+#pragma unroll
+    for (int u = 0; u < WR_CH * 64 / 256; ++u) *reinterpret_cast<f16*>(scl + (u * 256 + tid) * 2) = wl_factor(sb[u]);
+    for (int t = 0; t < n; ++t) {
+      if (t + WR_S - 2 < n) ea_wait_dma<(WR_S - 2) * 6>();           // (step t + WR_S - 2 has been issued: it alone may be in flight)
+      else ea_wait_dma<0>();
+      ea_raw_barrier();
+      if (t + WR_S - 1 < n) stage(t + WR_S - 1);
+      const char* buf = smem + (t % WR_S) * WR_STEP;
+      f16x8 sc[2], fa[4][2], fx[4][2];
+      u32x2 w[2][2];
+      sc[0] = *reinterpret_cast<const f16x8*>(scl + (t * 64 + 8 * lq) * 2);
+      sc[1] = *reinterpret_cast<const f16x8*>(scl + (t * 64 + 32 + 8 * lq) * 2);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        wl_read_x<0>(buf + ax[2 * h], buf + ax[2 * h + 1], w);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) fx[2 * h + j][ks] = wl_decode8(w[j][ks], sc[ks]);
       }
-      if (tk == 0 && wk == 0 && l15 == 0) db[n] = accb[i][r];
+      wl_read_d<0>(buf + ad[0], buf + ad[1], buf + ad[2], buf + ad[3], fa);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = ea_mfma_16x16x32(fx[j][ks], fa[i][ks], acc[i][j]);
+        if (sums) {
+          accb = ea_mfma_16x16x32(wl_unit_row(0, l15), fa[0][ks], accb);
+          accb = ea_mfma_16x16x32(wl_unit_row(1, l15), fa[1][ks], accb);
+        }
+      }
+    }
+  }
+  float* dw = p.dw + (long long)blockIdx.y * p.part;
+  float* db = p.splits > 1 ? dw + (long long)p.N * p.K : p.db;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {            // D^T: a lane holds 4 consecutive k of one n
+    const int n = n0 + wm * 64 + (i ^ (2 * wn)) * 16 + l15;
+    if (n >= p.N) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wn * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
+    if (i < 2 && sums && lq == 0) db[n] = accb[i];
+  }
+}
+
+__global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams p) {
+  EA_SMEM(smem);
+  const int tid = threadIdx.x, lane = tid & 63, wave = ea_uniform(tid >> 6), wm = wave >> 2, wn = wave & 3;
+  const int l15 = lane & 15, lq = lane >> 4;
+  int tn, tk;
+  {   // an XCD's workgroups share dy columns and x columns: one contiguous run of tiles, all k tiles of an n tile first
+    const int n = p.tiles_n * p.tiles_k, q = n >> 3, r = n & 7, xcd = blockIdx.x & 7;
+    const int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
+    tn = ea_uniform(t / p.tiles_k);
+    tk = ea_uniform(t - tn * p.tiles_k);
+  }
+  const int n0 = tn * 256, k0 = tk * 256;
+  const int m_begin = blockIdx.y * p.rows_per_split;
+  const int m_end = m_begin + p.rows_per_split < p.M ? m_begin + p.rows_per_split : p.M;
+  const int steps = (m_end - m_begin + 63) >> 6;
+
+  // DMA: dy half h, instruction i of this wave: rows 4 (2 wave + i) ... + 3 (256 bytes each: columns 64 h of wave row 0, then of wave row 1);
+  // x half h: rows 8 wave ... + 7 (128 bytes each: 32 h of the four wave columns)
+  unsigned vd[2][2], vx[2];                // columns that are not there start at 2 GiB, behind every descriptor
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 4 * (2 * wave + i) + (lane >> 4), piece = ((lane & 15) >> 1) ^ wl_dy_swz(r);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = (piece >> 2) * 128 + h * 64 + (piece & 3) * 16 + (lane & 1) * 8;
+      vd[h][i] = n0 + c < p.N ? ((unsigned)r * (unsigned)p.N + (unsigned)c) * 2u : EA_F8_NOWHERE;
+    }
+  }
+  {
+    const int r = 8 * wave + (lane >> 3), piece = (lane & 7) ^ wl_x_swz(r);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = (piece >> 1) * 64 + h * 32 + (piece & 1) * 16;
+      vx[h] = k0 + c < p.Kp ? (unsigned)r * (unsigned)p.Kp + (unsigned)c : EA_F8_NOWHERE;
+    }
+  }
+  char* sbuf = smem;
+  unsigned od = 0, ox = 0;
+  // descriptors of a chunk: from its first row to the slice's last one (rows behind it read as zeros)
+  ea_rows rd = ea_make_rows(p.dy, 0), rx = ea_make_rows(p.x, 0);
+  int t0 = 0;                              // the chunk's first step
+  auto begin = [&](int t) {                // t: step of the chunk
+    sbuf = smem + (t & 1) * WL_STEP;
+    od = ea_uniform((unsigned)t * 64u * (unsigned)p.N * 2u);
+    ox = ea_uniform((unsigned)t * 64u * (unsigned)p.Kp);
+  };
+  auto stage_d = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wl_dma16(rd, vd[h][i] + od, sbuf + h * 16384 + (2 * wave + i) * 1024);
+  };
+  auto stage_x = [&](int h) { wl_dma16(rx, vx[h] + ox, sbuf + WL_DY + h * 8192 + wave * 1024); };
+
+  f32x4 acc[8][4], accb = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  f16x8 fa[4][2];
+  f16x8 fb0[2][2], fb1[2][2], fbn[2][2];  // quadrants 0 and 1, the next step's 0
+  // rows 8 lq ... + 7 of a 32-row half of the step are this lane group's share of one MFMA, for both operands.  The swizzle does not
+  // change over the 32-row halves or the 4-row quarters of a group: one address per fragment, the rest are immediate offsets
+  // (fragment i is the quadrant's 16-column group i ^ wn: each wave column sums dy over the group of its own fragment 0)
+  int ad[4], ax[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * lq + (l15 >> 2);
+    ad[i] = r * 256 + (((wm * 4 + (i ^ wn)) ^ wl_dy_swz(r)) << 5) + (l15 & 3) * 8;
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = 8 * lq + (l15 >> 1);
+    ax[j] = WL_DY + r * 128 + (((wn * 2 + j) ^ wl_x_swz(r)) << 4) + (l15 & 1) * 8;
+  }
+  auto read_d = [&](const char* buf, auto qa_c) { wl_read_d<decltype(qa_c)::value * 16384>(buf + ad[0], buf + ad[1], buf + ad[2], buf + ad[3], fa); };
+  constexpr std::integral_constant<int, 0> c0{};
+  constexpr std::integral_constant<int, 1> c1{};
+  char* const scl = smem + WL_SCL;         // [step of the chunk][kb of the tile][64]
+  auto read_x = [&](int t, auto qb_c, f16x8 (&f)[2][2]) {          // codes and factors of one quadrant -> fragments
+    const char* buf = smem + (t & 1) * WL_STEP;
+    f16x8 sc[2];
+    u32x2 w[2][2];
+    sc[0] = *reinterpret_cast<const f16x8*>(scl + (t * 128 + (wn >> 1) * 64 + 8 * lq) * 2);
+    sc[1] = *reinterpret_cast<const f16x8*>(scl + (t * 128 + (wn >> 1) * 64 + 32 + 8 * lq) * 2);
+    wl_read_x<decltype(qb_c)::value * 8192>(buf + ax[0], buf + ax[1], w);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) f[j][ks] = wl_decode8(w[j][ks], sc[ks]);
+  };
+  auto mma = [&](auto qa_c, auto qb_c, const f16x8 (&fb)[2][2], bool sums) {
+    constexpr int qa = decltype(qa_c)::value, qb = decltype(qb_c)::value;
+#ifndef EA_EMU
+    __builtin_amdgcn_s_setprio(1);
+#endif
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[qa * 4 + i][qb * 2 + j] = ea_mfma_16x16x32(fb[j][ks], fa[i][ks], acc[qa * 4 + i][qb * 2 + j]);
+      if (sums) {                          // row qa of the other operand is ones: D's row qa is the column sums of quadrant qa
+        accb = ea_mfma_16x16x32(wl_unit_row(qa, l15), fa[0][ks], accb);
+      }
+    }
+#ifndef EA_EMU
+    __builtin_amdgcn_s_setprio(0);
+#endif
+  };
+  const bool sums = tk == 0;
+  auto body = [&](int t, auto more_c) {
+    constexpr bool more = decltype(more_c)::value;
+    const char* buf = smem + (t & 1) * WL_STEP;
+    if (more) { begin(t + 1); stage_x(0); stage_x(1); }
+    read_d(buf, c0);
+    if (more) ea_wait_dma<2>(); else ea_wait_dma<0>();
+    ea_f8l_barrier();
+    mma(c0, c0, fb0, sums);
+    ea_f8l_barrier();
+    if (more) stage_d(0);
+    read_x(t, c1, fb1);
+    if (more) ea_wait_dma<4>();
+    ea_f8l_barrier();
+    mma(c0, c1, fb1, false);
+    ea_f8l_barrier();
+    if (more) stage_d(1);
+    read_d(buf, c1);
+    if (more) ea_wait_dma<4>();
+    ea_f8l_barrier();
+    mma(c1, c1, fb1, sums);
+    ea_f8l_barrier();
+    if (more) {
+      read_x(t + 1, c0, fbn);
+      ea_wait_dma<2>();
+    }
+    ea_f8l_barrier();
+    mma(c1, c0, fb0, false);
+    if (more)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) fb0[j][ks] = fbn[j][ks];
+    ea_f8l_barrier();
+  };
+  for (; t0 < steps; t0 += WL_CH) {
+    const int n = steps - t0 < WL_CH ? steps - t0 : WL_CH;
+    const long long mc = m_begin + t0 * 64ll;
+    if (t0) ea_raw_barrier();              // the chunk before this one has been read
+    unsigned char sb[WL_CH * 128 / 512];
+    int kb = 2 * tk + ((tid >> 6) & 1);
+    if (kb >= (p.Kp >> 7)) kb = (p.Kp >> 7) - 1;
+    const int mt = (tid >> 7) * 64 + (tid & 63), left = (int)(m_end - mc);
+    const uint8_t* const sx = p.sx + kb * p.Rp + mc + mt;
+#pragma unroll
+    for (int u = 0; u < WL_CH * 128 / 512; ++u) sb[u] = mt + u * 256 < left ? sx[u * 256] : 0;      // (a row that is not there: factor 0)
+    rd = ea_make_rows(p.dy + mc * p.N + n0, ((m_end - mc) * p.N - n0) * 2);
+    rx = ea_make_rows(p.x + mc * p.Kp + k0, (m_end - mc) * p.Kp - k0);
+    begin(0);
+    stage_x(0);
+    stage_x(1);
+    stage_d(0);
+    stage_d(1);
+#pragma unroll
+    for (int u = 0; u < WL_CH * 128 / 512; ++u) *reinterpret_cast<f16*>(scl + (u * 512 + tid) * 2) = wl_factor(sb[u]);
+    ea_wait_dma<2>();
+    ea_raw_barrier();
+    read_x(0, c0, fb0);
+    if (wm == 1) ea_f8l_barrier();         // wave row 1 runs one barrier behind wave row 0
+    for (int t = 0; t + 1 < n; ++t) body(t, std::true_type{});
+    body(n - 1, std::false_type{});
+    if (wm == 0) ea_f8l_barrier();         // both wave rows execute the same number of barriers
+  }
+  float* dw = p.dw + (long long)blockIdx.y * p.part;
+  float* db = p.splits > 1 ? dw + (long long)p.N * p.K : p.db;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {            // D^T: a lane holds 4 consecutive k of one n
+    const int n = n0 + wm * 128 + (i >> 2) * 64 + ((i & 3) ^ wn) * 16 + l15;
+    if (n >= p.N) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wn * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
+  }
+  if (sums && lq == 0)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int n = n0 + wm * 128 + q * 64 + wn * 16 + l15;
+      if (n < p.N) db[n] = accb[q];
     }
 }
 
 // sum of the slices, in their order
-__global__ __launch_bounds__(256) void ea_fp8_wgrad_join_kernel(const float* part, float* dw, float* db, long long nk, long long total, int splits) {
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+__global__ __launch_bounds__(64) void ea_fp8_wgrad_join_kernel(const float* part, float* dw, float* db, long long nk, long long total, int splits) {
+  const long long i = ((long long)blockIdx.x * 64 + threadIdx.x) * 4;
   if (i >= total) return;
   const long long left = total - i;
   f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int t = 0; t < splits; ++t) {
-    const float* q = part + t * ((total + 3) & ~3ll) + i;          // (slices are padded to whole vectors)
-    s += *reinterpret_cast<const f32x4*>(q);
-  }
+#pragma unroll 8
+  for (int t = 0; t < splits; ++t) s += *reinterpret_cast<const f32x4*>(part + t * ((total + 3) & ~3ll) + i);      // (slices are padded to whole vectors)
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (j < left) (i + j < nk ? dw[i + j] : db[i + j - nk]) = s[j];
 }
 
-int wgrad_splits(int M, int N, int K) {
-  const int tiles = ((N + WG_T - 1) / WG_T) * ((K + WG_T - 1) / WG_T), steps = (M + WG_R - 1) / WG_R;
-  int s = tiles >= 512 ? 1 : 512 / tiles;
-  if (s > steps / 4) s = steps / 4;
-  return s < 1 ? 1 : s;
+// Kernel (256, 128: the DMA kernels; 0: the one for any N and alignment) and number of slices of the rows: the least time by a model of
+// what was measured.  A 64-row step takes a 256 x 256 workgroup 1.65 us, a 128 x 128 one 0.87 us alone on its CU and 1.25 us beside
+// another; a workgroup's start and end 10 / 5 us; joining s slices 4 us and 2 s + 1 passes over the output at 8 TB/s.
+//   16384 x 1280 x 5120 (M x N x K): 256 with 5 slices 220 us (2: 225, 1: 400; 128: 263 at best), 32768 x 2560 x 320: 256 with 12 slices 89
+//   (128 with 8: 103), 8192 x 640 x 640: 128 with 10 slices 25 (1: 111; 256 with 24: 32), 616 x 1280 x 1024: 128 with 1 slice 14 (2: 19; 256: 27)
+// Workspace and launch go by the same answer, which depends on the sizes alone.
+struct WgradPlan { int kernel, splits, rows; };
+WgradPlan wgrad_plan(int M, int N, int K) {
+  WgradPlan w{-1, 1, 64};
+  const int v = ea_forced_variant();       // tests: 101, 102, 103 pin a kernel
+  const bool dma = (N & 7) == 0 && N <= (1 << 18) && K <= (1 << 18) && v != 103;
+  const double nk = (double)N * K;
+  const int steps = (M + 63) / 64;
+  double best = 0;
+  for (int kernel = 256; kernel >= 0; kernel -= 128) {
+    if (kernel ? !dma || (v == 101 && kernel != 256) || (v == 102 && kernel != 128) : dma) continue;
+    const int tile = kernel == 256 ? 256 : 128;
+    const long long tiles = (long long)((N + tile - 1) / tile) * ((K + tile - 1) / tile);
+    for (int s = 1; s <= steps && s <= 64; ++s) {
+      const int per = (steps + s - 1) / s;
+      if ((steps + per - 1) / per != s) continue;                    // (this many slices leave one empty)
+      const long long wgs = tiles * s;
+      const double t = (kernel == 256 ? (wgs + 255) / 256 * (per * 1.65 + 10)
+                                      : wgs / 512 * (per * 1.25 + 5) + (wgs % 512 > 256 ? per * 1.25 + 5 : wgs % 512 ? per * 0.87 + 5 : 0)) +
+                       (s > 1 ? 4 + (2 * s + 1) * nk * 4 / 8e6 : 0);
+      if (w.kernel < 0 || t < best) {
+        best = t;
+        w = WgradPlan{kernel, s, per * 64};
+      }
+    }
+  }
+  return w;
 }
 
 long long fp8_tiles(const EaFp8GemmParams& p, int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); }
@@ -232,7 +694,7 @@ extern "C" int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const vo
 
 extern "C" size_t ea_gemm_fp8_wgrad_workspace_bytes(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const int s = wgrad_splits(M, N, K);
+  const int s = wgrad_plan(M, N, K).splits;
   return s == 1 ? 0 : (size_t)s * ((((size_t)N * K + N) + 3) & ~(size_t)3) * sizeof(float);
 }
 
@@ -244,25 +706,36 @@ extern "C" int ea_gemm_fp8_wgrad(const void* dy, const void* x, const unsigned c
   if (ws_bytes < ea_gemm_fp8_wgrad_workspace_bytes(M, N, K) || (!workspace && ws_bytes)) return EA_ERR_WORKSPACE;
   WgradParams p;
   memset(&p, 0, sizeof(p));
-  p.splits = wgrad_splits(M, N, K);
+  const WgradPlan w = wgrad_plan(M, N, K);
+  p.splits = w.splits;
+  p.rows_per_split = w.rows;
   if (p.splits > 1 && !workspace) return EA_ERR_WORKSPACE;
-  const int steps = (M + WG_R - 1) / WG_R;
-  p.rows_per_split = (steps + p.splits - 1) / p.splits * WG_R;
+  const int kernel = ((uintptr_t)dy & 15) ? 0 : w.kernel, tile = kernel == 256 ? 256 : 128;
   p.dy = (const f16*)dy; p.x = (const uint8_t*)x; p.sx = x_scale;
   p.M = M; p.N = N; p.K = K; p.Kp = ea_fp8_blocks(K) * EA_FP8_BLOCK; p.Rp = ea_fp8_scale_pitch(M);
-  p.tiles_n = (N + WG_T - 1) / WG_T; p.tiles_k = (K + WG_T - 1) / WG_T;
+  p.tiles_n = (N + tile - 1) / tile; p.tiles_k = (K + tile - 1) / tile;
   p.part = p.splits > 1 ? (((long long)N * K + N + 3) & ~3ll) : 0;
   p.dw = p.splits > 1 ? (float*)workspace : dw;
   p.db = db;
   p.vec = (N & 7) == 0 && ((uintptr_t)dy & 15) == 0;
   const long long tiles = (long long)p.tiles_n * p.tiles_k;
   if (tiles > 0x7fffffffll) return EA_ERR_BAD_SHAPE;
-  auto k = ea_fp8_wgrad_kernel;
-  EA_LAUNCH(k, dim3((unsigned)tiles, p.splits), dim3(256), 2 * WG_BUF, stream, p);
+  if (kernel == 256) {
+    auto k = ea_fp8_wgrad_large_kernel;
+    ea_allow_big_lds(k, WL_LDS);
+    EA_LAUNCH(k, dim3((unsigned)tiles, p.splits), dim3(512), WL_LDS, stream, p);
+  } else if (kernel == 128) {
+    auto k = ea_fp8_wgrad_ring_kernel;
+    ea_allow_big_lds(k, WR_LDS);
+    EA_LAUNCH(k, dim3((unsigned)tiles, p.splits), dim3(256), WR_LDS, stream, p);
+  } else {
+    auto k = ea_fp8_wgrad_kernel;
+    EA_LAUNCH(k, dim3((unsigned)tiles, p.splits), dim3(256), 2 * WG_BUF, stream, p);
+  }
   int st = ea_launch_status();
   if (st != EA_OK || p.splits == 1) return st;
   auto j = ea_fp8_wgrad_join_kernel;
   const long long total = (long long)N * K + N;
-  EA_LAUNCH(j, dim3((unsigned)((total + 1023) / 1024)), dim3(256), 0, stream, (const float*)workspace, dw, db, (long long)N * K, total, p.splits);
+  EA_LAUNCH(j, dim3((unsigned)((total + 255) / 256)), dim3(64), 0, stream, (const float*)workspace, dw, db, (long long)N * K, total, p.splits);
   return ea_launch_status();
 }

@@ -500,8 +500,11 @@ def test_gemm_fp8_residual_may_be_the_output(kb):
 
 
 # ------------------------------------------------------------------------------------------------------------ weight gradient
-@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 8, 128), (64, 128, 128), (70, 100, 300), (130, 136, 77), (333, 24, 200), (600, 130, 129), (65, 7, 640)])
-def test_gemm_fp8_wgrad(kb, M, N, K):
+@pytest.mark.parametrize("kernel", [0, 101, 102, 103])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 8, 128), (64, 128, 128), (70, 104, 300), (130, 136, 77), (333, 24, 200), (600, 130, 129), (65, 7, 640),
+                                   (2250, 264, 260)])
+def test_gemm_fp8_wgrad(kb, M, N, K, kernel):
+    force(kb, kernel)
     q, e = quantize(rows(17, M, K, np.float32))
     dy = rows(18, M, N, np.float16, 0.05)
     dw, db = kb.up(np.full((N + 1, K), 7, np.float32)), kb.up(np.full((N + 1,), 7, np.float32))

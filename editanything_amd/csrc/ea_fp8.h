@@ -17,13 +17,14 @@
 #define EA_FP8_BLOCK 128
 #define EA_FP8_E_MIN (-100)
 #define EA_FP8_E_MAX 120
+#define EA_INF_BITS 0x7f800000u
 
 __device__ __forceinline__ unsigned ea_f2u(float v) { return __builtin_bit_cast(unsigned, v); }
 __device__ __forceinline__ float ea_u2f(unsigned v) { return __builtin_bit_cast(float, v); }
 // |v| where it enters a block's maximum: NaN and infinity count as 0
 __device__ __forceinline__ float ea_finite_abs(float v) {
   const unsigned u = ea_f2u(v) & 0x7fffffffu;
-  return u < 0x7f800000u ? ea_u2f(u) : 0.0f;
+  return u < EA_INF_BITS ? ea_u2f(u) : 0.0f;
 }
 // the block's exponent byte from its maximum: 448 = 1.75 * 2^8
 __device__ __forceinline__ int ea_fp8_exp_byte(float amax) {
@@ -73,16 +74,9 @@ __device__ __forceinline__ void ea_fp8_unpack4(unsigned w, float* v) {
   v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
 }
 #endif
-// x * 2^-E ready for the conversion: what is not finite becomes a NaN code
+// x * 2^-E for the conversion: what is not finite becomes a NaN code
 __device__ __forceinline__ float ea_fp8_prep(float x, float inv) {
-  return (ea_f2u(x) & 0x7fffffffu) < 0x7f800000u ? x * inv : ea_u2f(0x7fc00000u);
-}
-// 8 values -> 8 codes
-__device__ __forceinline__ u32x2 ea_fp8_encode8(const float* v, float inv) {
-  float t[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) t[j] = ea_fp8_prep(v[j], inv);
-  return u32x2{ea_fp8_pack4(t[0], t[1], t[2], t[3]), ea_fp8_pack4(t[4], t[5], t[6], t[7])};
+  return (ea_f2u(x) & 0x7fffffffu) < EA_INF_BITS ? x * inv : ea_u2f(0x7fc00000u);
 }
 
 // ---- reductions over aligned groups of LPR lanes (8, 16, 32, 64); every lane gets the result.  Up to 16 lanes they stay in the
@@ -113,6 +107,102 @@ __device__ __forceinline__ float ea_group_sum(float v) {
 template <int LPR>
 __device__ __forceinline__ float ea_group_max(float v) {
   return ea_group_reduce<LPR>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
+template <int LPR>
+__device__ __forceinline__ unsigned ea_group_max_bits(unsigned v) {        // of |v|'s bits: their order is that of the values
+  return ea_f2u(ea_group_reduce<LPR>(ea_u2f(v), [](float a, float b) { return ea_f2u(a) > ea_f2u(b) ? a : b; }));
+}
+// does any lane of the wave say so?
+__device__ __forceinline__ bool ea_any(bool c) {
+#ifdef EA_EMU
+  char* s = ea_emu::wave_scratch();
+  s[ea_emu::lane_id() * 64] = c;
+  ea_emu::wave_sync();
+  bool r = false;
+  for (int l = 0; l < ea_emu::wave_lanes(); ++l) r = r || s[l * 64];
+  ea_emu::wave_sync();
+  return r;
+#else
+  return __builtin_amdgcn_ballot_w64(c) != 0;
+#endif
+}
+
+// ---- encoding 8 finite values with their block's exponent byte: one instruction for two values, the power of two included
+__device__ __forceinline__ u32x2 ea_fp8_pack8(const float* v, int byte) {
+#ifdef EA_EMU
+  const float f = ea_fp8_inv_scale(byte);
+  return u32x2{ea_fp8_pack4(v[0] * f, v[1] * f, v[2] * f, v[3] * f), ea_fp8_pack4(v[4] * f, v[5] * f, v[6] * f, v[7] * f)};
+#else
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  const float f = ea_fp8_scale(byte);
+  s16x2 a = {0, 0}, b = {0, 0};
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(a, v[0], v[1], f, false);
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(a, v[2], v[3], f, true);
+  b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(b, v[4], v[5], f, false);
+  b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(b, v[6], v[7], f, true);
+  return u32x2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+#endif
+}
+__device__ __forceinline__ u32x2 ea_fp8_pack8(f16x8 v, int byte) {
+#ifdef EA_EMU
+  float t[8];
+  for (int j = 0; j < 8; ++j) t[j] = (float)v[j];
+  return ea_fp8_pack8(t, byte);
+#else
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  typedef __fp16 h2 __attribute__((ext_vector_type(2)));
+  const float f = ea_fp8_scale(byte);
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  const unsigned w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
+  s16x2 a = {0, 0}, b = {0, 0};
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(a, __builtin_bit_cast(h2, w0), f, false);
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(a, __builtin_bit_cast(h2, w1), f, true);
+  b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, __builtin_bit_cast(h2, w2), f, false);
+  b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, __builtin_bit_cast(h2, w3), f, true);
+  return u32x2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+#endif
+}
+// the largest |v| of 8 values, as fp32 bits (at least EA_INF_BITS where one of them is not finite)
+__device__ __forceinline__ unsigned ea_max_bits8(const float* v) {
+  unsigned m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned u = ea_f2u(v[j]) & 0x7fffffffu;
+    m = u > m ? u : m;
+  }
+  return m;
+}
+__device__ __forceinline__ unsigned ea_max_bits8(f16x8 v) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  const unsigned a0 = w[0] & 0x7fff7fffu, a1 = w[1] & 0x7fff7fffu, a2 = w[2] & 0x7fff7fffu, a3 = w[3] & 0x7fff7fffu;
+  const u16x2 p = __builtin_elementwise_max(__builtin_bit_cast(u16x2, a0), __builtin_bit_cast(u16x2, a1));
+  const u16x2 q = __builtin_elementwise_max(__builtin_bit_cast(u16x2, a2), __builtin_bit_cast(u16x2, a3));
+  const u16x2 m = __builtin_elementwise_max(p, q);
+  const unsigned short h = m[0] > m[1] ? m[0] : m[1];
+  return ea_f2u((float)__builtin_bit_cast(f16, h)) & 0x7fffffffu;
+}
+// One block of 128: 16 lanes (GRP; 8 columns each) turn their 8 values into codes and the block's exponent byte.  Every lane of the wave
+// calls it.  Blocks with values that are not finite take the slow way: those become NaN codes and stay out of the maximum.
+template <int GRP, typename V>
+__device__ __forceinline__ u32x2 ea_fp8_block(const V& v, int& byte) {
+  const unsigned m = ea_group_max_bits<GRP>(ea_max_bits8(v));
+  if (!ea_any(m >= EA_INF_BITS)) {
+    byte = ea_fp8_exp_byte(ea_u2f(m));
+    return ea_fp8_pack8(v, byte);
+  }
+  float t[8], top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    t[j] = (float)v[j];
+    top = fmaxf(top, ea_finite_abs(t[j]));
+  }
+  byte = ea_fp8_exp_byte(ea_group_max<GRP>(top));
+  const float inv = ea_fp8_inv_scale(byte);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = ea_fp8_prep(t[j], inv);
+  return u32x2{ea_fp8_pack4(t[0], t[1], t[2], t[3]), ea_fp8_pack4(t[4], t[5], t[6], t[7])};
 }
 
 static inline int ea_fp8_blocks(int cols) { return (cols + EA_FP8_BLOCK - 1) / EA_FP8_BLOCK; }

@@ -7,11 +7,15 @@
 // All sums and statistics are fp32; the variance is the centred one (two passes over registers).  x is fp16, fp32 or an 8-bit
 // tensor (ea_fp8.h); the forward's y is fp16 or goes straight into the 8-bit format.
 //
-// Both passes read every operand once and are bound by HBM.  A row belongs to LPR lanes (8 ... 64: a 320-wide row is 40 16-byte
-// vectors, which would leave 24 of 64 lanes idle), so a wave holds 64 / LPR rows whole in registers; the row sums are DPP steps.
+// Both passes read every operand once and are bound by HBM.  A row belongs to LPR lanes (16, 32 or 64), so a wave holds 64 / LPR rows
+// whole in registers; the row sums are DPP steps.  The fewest lanes that hold a row in three 16-byte vectors each: 8 lanes with six
+// vectors keep every lane of a 320-wide row busy, but their 240 registers of sums and row leave one wave per SIMD and their end is long
+// (backward 32768 x 320: 55 us against 23).
 // The column sums stay in registers over all rows that a wave visits (a lane always owns the same columns), are joined over the
 // workgroup in LDS once, written as one partial per workgroup and joined by a second launch in a fixed order: no atomics, so a
-// run repeats bit for bit.
+// run repeats bit for bit.  Measured (backward with residual): 16384 x 1280 fp32 52 us = 5.7 TB/s, 32768 x 1280 fp16 without residual
+// 45 us = 5.6 TB/s, 32768 x 320 fp16 23 us = 3.7 TB/s, 512 x 1280 9 us (two launches).  Forward: 32768 x 1280 fp16 30 us = 5.6 TB/s, into
+// 8 bits 28 us.  The next row is in flight while one is worked off (without: 16384 x 1280 64 us).
 #include "ea_fp8.h"
 #include "../../include/editanything_hip.h"
 
@@ -103,20 +107,15 @@ __global__ __launch_bounds__(256) void ea_ln_train_kernel(LnTrainParams p) {
   }
   const float rstd = 1.0f / sqrtf(ea_group_sum<LPR>(q) / (float)p.C + p.eps);
   if (row < p.M && l == 0) *reinterpret_cast<f32x2*>(p.stats + 2ll * row) = f32x2{mean, rstd};
-  float bmax[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (l + LPR * i) * VEC;
-    bmax[i] = 0.0f;
     if (c < p.C) {
       float ga[VEC], be[VEC];
       ld_f32<VEC>(p.gamma + c, ga);
       ld_f32<VEC>(p.beta + c, be);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        x[i][j] = (x[i][j] - mean) * rstd * ga[j] + be[j];
-        bmax[i] = fmaxf(bmax[i], ea_finite_abs(x[i][j]));
-      }
+      for (int j = 0; j < VEC; ++j) x[i][j] = (x[i][j] - mean) * rstd * ga[j] + be[j];
       if (!OUT8 && row < p.M) {
         f16* o = p.y + (long long)row * p.C + c;
         if constexpr (VEC == 8) {
@@ -129,25 +128,30 @@ __global__ __launch_bounds__(256) void ea_ln_train_kernel(LnTrainParams p) {
     }
   }
   if constexpr (OUT8) {
-    // a block of 128 columns: 16 lanes of one vector (LPR >= 16), or PAIR vectors of the whole group (8 lanes; 64 scalars)
-    constexpr int PAIR = (VEC == 1 || LPR == 8) ? 2 : 1;
-    constexpr int GRP = VEC == 1 ? 64 : (LPR < 16 ? LPR : 16);
-    static_assert(NV % PAIR == 0, "a block's vectors come in pairs");
+    // a block of 128 columns: 16 lanes of one vector, or two scalars of the whole wave
+    if constexpr (VEC == 8) {
 #pragma unroll
-    for (int i = 0; i < NV; i += PAIR) {
-      float m = bmax[i];
-      if (PAIR == 2) m = fmaxf(m, bmax[i + PAIR - 1]);
-      m = ea_group_max<GRP>(m);
-      const int e = ea_fp8_exp_byte(m);
-      const float inv = ea_fp8_inv_scale(e);
-#pragma unroll
-      for (int u = 0; u < PAIR; ++u) {
-        const int c = (l + LPR * (i + u)) * VEC;
+      for (int i = 0; i < NV; ++i) {
+        const int c = (l + LPR * i) * 8;
+        int e;
+        const u32x2 w = ea_fp8_block<16>((const float*)x[i], e);
         if (row < p.M && c < p.Kp) {
-          uint8_t* o = p.q + (long long)row * p.Kp + c;
-          if constexpr (VEC == 8) *reinterpret_cast<u32x2*>(o) = ea_fp8_encode8(x[i + u], inv);
-          else *o = (uint8_t)ea_fp8_pack4(ea_fp8_prep(x[i + u][0], inv), 0.0f, 0.0f, 0.0f);
+          *reinterpret_cast<u32x2*>(p.q + (long long)row * p.Kp + c) = w;
           if ((c & 127) == 0) p.scale[(long long)(c >> 7) * p.Rp + row] = (uint8_t)e;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; i += 2) {
+        const int e = ea_fp8_exp_byte(ea_group_max<64>(fmaxf(ea_finite_abs(x[i][0]), ea_finite_abs(x[i + 1][0]))));
+        const float inv = ea_fp8_inv_scale(e);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int c = l + 64 * (i + u);
+          if (row < p.M && c < p.Kp) {
+            p.q[(long long)row * p.Kp + c] = (uint8_t)ea_fp8_pack4(ea_fp8_prep(x[i + u][0], inv), 0.0f, 0.0f, 0.0f);
+            if ((c & 127) == 0) p.scale[(long long)(c >> 7) * p.Rp + row] = (uint8_t)e;
+          }
         }
       }
     }
@@ -157,15 +161,60 @@ __global__ __launch_bounds__(256) void ea_ln_train_kernel(LnTrainParams p) {
 // ----------------------------------------------------------------------------------------------------------- backward
 struct LnBwdParams {
   const f16* dy; const void* x; const uint8_t* x_scale; const float* stats; const float* gamma;
-  const void* residual; void* dx; int dx_f32;          // residual and dx share a type
+  const void* residual; void* dx;
   float* part;                         // [gridDim.x][2][C]
   int M, C, xpitch; long long xspitch;
 };
 
-template <int XK, int VEC, int LPR, int NV>
+// VEC values as they lie in memory: loaded a row ahead, converted when they are used
+template <int XK, int VEC>
+struct Raw {
+  u32x4 a, b;                          // (fp32: both; fp16: a; codes: half of a and the scale byte in a[2])
+  __device__ __forceinline__ void load(const void* x, const uint8_t* scale, long long row, int pitch, long long spitch, int c) {
+    if constexpr (XK == XK_F16) {
+      a = *reinterpret_cast<const u32x4*>((const f16*)x + row * pitch + c);
+    } else if constexpr (XK == XK_F32) {
+      a = *reinterpret_cast<const u32x4*>((const float*)x + row * pitch + c);
+      b = *reinterpret_cast<const u32x4*>((const float*)x + row * pitch + c + 4);
+    } else {
+      const u32x2 w = *reinterpret_cast<const u32x2*>((const uint8_t*)x + row * pitch + c);
+      a[0] = w[0];
+      a[1] = w[1];
+      a[2] = scale[(long long)(c >> 7) * spitch + row];
+    }
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    if constexpr (XK == XK_F16) {
+      const f16x8 h = __builtin_bit_cast(f16x8, a);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+    } else if constexpr (XK == XK_F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = ea_u2f(j < 4 ? a[j & 3] : b[j & 3]);
+    } else {
+      const float s = ea_fp8_scale((int)a[2]);
+      ea_fp8_unpack4(a[0], v);
+      ea_fp8_unpack4(a[1], v + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= s;
+    }
+  }
+};
+template <int XK>
+struct Raw<XK, 1> {
+  float a;
+  __device__ __forceinline__ void load(const void* x, const uint8_t* scale, long long row, int pitch, long long spitch, int c) {
+    ld_row<XK, 1>(x, scale, row, pitch, spitch, c, &a);
+  }
+  __device__ __forceinline__ void get(float* v) const { v[0] = a; }
+};
+
+// F32: the type of residual and dx
+template <int XK, bool F32, int VEC, int LPR, int NV>
 __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
   constexpr int RPW = 64 / LPR;
-  constexpr bool KEEP = NV <= 24;      // more scalars per lane than that do not fit in registers twice: the row is read again (from L2)
+  constexpr int RK = F32 ? XK_F32 : XK_F16;
+  constexpr bool KEEP = NV * VEC <= 24;      // a lane's share of a row stays in registers; a larger one is loaded twice, the second time from L2
   EA_SMEM(smem);
   float* red = reinterpret_cast<float*>(smem);      // [4][C]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, l = lane % LPR;
@@ -179,33 +228,50 @@ __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
   }
   const float inv_c = 1.0f / (float)p.C;
   const long long stride = (long long)gridDim.x * 4 * RPW;
-  for (long long base = ((long long)blockIdx.x * 4 + wave) * RPW; base < p.M; base += stride) {
+  constexpr int NR = KEEP ? NV : 1;
+  Raw<XK, VEC> rx[NR];
+  Raw<XK_F16, VEC> ry[NR];
+  Raw<RK, VEC> rr[NR];
+  f32x2 st;
+  auto fetch1 = [&](long long row, int i, int k) {           // clamped, unconditional: the whole row's loads are in flight together
+    const int c0 = (l + LPR * i) * VEC, c = c0 < p.C ? c0 : 0;
+    rx[k].load(p.x, p.x_scale, row, p.xpitch, p.xspitch, c);
+    ry[k].load(p.dy, nullptr, row, p.C, 0, c);
+  };
+  auto fetch_res = [&](long long row, int i, int k) {
+    const int c0 = (l + LPR * i) * VEC, c = c0 < p.C ? c0 : 0;
+    rr[k].load(p.residual, nullptr, row, p.C, 0, c);
+  };
+  auto fetch = [&](long long base) {
+    const long long r = base + sub < p.M ? base + sub : p.M - 1;
+    st = *reinterpret_cast<const f32x2*>(p.stats + 2 * r);
+    if (KEEP)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) fetch1(r, i, KEEP ? i : 0);
+  };
+  long long base = ((long long)blockIdx.x * 4 + wave) * RPW;
+  if (base < p.M) fetch(base);
+  for (; base < p.M; base += stride) {
     const long long row = base + sub;
     const bool live = row < p.M;
     const long long r = live ? row : p.M - 1;
-    const f32x2 st = *reinterpret_cast<const f32x2*>(p.stats + 2 * r);
-    float n[KEEP ? NV : 1][VEC], g[KEEP ? NV : 1][VEC];
+    const float mean = st[0], rs = st[1];
+    float n[NR][VEC], g[NR][VEC];
     float s1 = 0.0f, s2 = 0.0f;
-    auto load = [&](int c, float* nv, float* gv) {
-      if (c < p.C) {
-        ld_row<XK, VEC>(p.x, p.x_scale, r, p.xpitch, p.xspitch, c, nv);
-        ld_row<XK_F16, VEC>(p.dy, nullptr, r, p.C, 0, c, gv);
-      } else {
+    if (KEEP && p.residual)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) nv[j] = gv[j] = 0.0f;
-      }
-    };
-    if (KEEP)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) load((l + LPR * i) * VEC, n[KEEP ? i : 0], g[KEEP ? i : 0]);
+      for (int i = 0; i < NV; ++i) fetch_res(r, i, KEEP ? i : 0);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (l + LPR * i) * VEC, k = KEEP ? i : 0;
-      if (!KEEP) load(c, n[k], g[k]);
+      if (!KEEP) fetch1(r, i, 0);
+      rx[k].get(n[k]);
+      ry[k].get(g[k]);
+      const bool there = live && c < p.C;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float d = live && c < p.C ? g[k][j] : 0.0f;      // (a row or column that is not there adds nothing, whatever was read)
-        n[k][j] = live && c < p.C ? (n[k][j] - st[0]) * st[1] : 0.0f;
+        const float d = there ? g[k][j] : 0.0f;              // (a row or column that is not there adds nothing, whatever was read)
+        n[k][j] = there ? (n[k][j] - mean) * rs : 0.0f;
         ag[i][j] += d * n[k][j];
         ab[i][j] += d;
         g[k][j] = d * ga[i][j];
@@ -213,6 +279,7 @@ __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
         s2 += g[k][j] * n[k][j];
       }
     }
+    if (base + stride < p.M) fetch(base + stride);
     s1 = ea_group_sum<LPR>(s1) * inv_c;
     s2 = ea_group_sum<LPR>(s2) * inv_c;
     if (live) {
@@ -221,35 +288,36 @@ __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
         const int c = (l + LPR * i) * VEC, k = KEEP ? i : 0;
         if (c >= p.C) continue;
         if (!KEEP) {
-          load(c, n[k], g[k]);
+          fetch1(r, i, 0);
+          rx[0].get(n[0]);
+          ry[0].get(g[0]);
+          if (p.residual) fetch_res(r, i, 0);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            n[k][j] = (n[k][j] - st[0]) * st[1];
-            g[k][j] *= ga[i][j];
+            n[0][j] = (n[0][j] - mean) * rs;
+            g[0][j] *= ga[i][j];
           }
         }
         float o[VEC], res[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          o[j] = st[1] * (g[k][j] - s1 - n[k][j] * s2);
-          res[j] = 0.0f;
-        }
-        if (p.dx_f32) {
-          if (p.residual) ld_row<XK_F32, VEC>(p.residual, nullptr, row, p.C, 0, c, res);
+        for (int j = 0; j < VEC; ++j) res[j] = 0.0f;
+        if (p.residual) rr[k].get(res);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = rs * (g[k][j] - s1 - n[k][j] * s2) + res[j];
+        if constexpr (F32) {
           float* d = (float*)p.dx + row * p.C + c;
           if constexpr (VEC == 8) {
-            *reinterpret_cast<f32x4*>(d) = f32x4{o[0] + res[0], o[1] + res[1], o[2] + res[2], o[3] + res[3]};
-            *reinterpret_cast<f32x4*>(d + 4) = f32x4{o[4] + res[4], o[5] + res[5], o[6] + res[6], o[7] + res[7]};
-          } else *d = o[0] + res[0];
+            *reinterpret_cast<f32x4*>(d) = f32x4{o[0], o[1], o[2], o[3]};
+            *reinterpret_cast<f32x4*>(d + 4) = f32x4{o[4], o[5], o[6], o[7]};
+          } else *d = o[0];
         } else {
-          if (p.residual) ld_row<XK_F16, VEC>(p.residual, nullptr, row, p.C, 0, c, res);
           f16* d = (f16*)p.dx + row * p.C + c;
           if constexpr (VEC == 8) {
             f16x8 h;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = (f16)(o[j] + res[j]);
+            for (int j = 0; j < 8; ++j) h[j] = (f16)o[j];
             ea_st8(d, h);
-          } else *d = (f16)(o[0] + res[0]);
+          } else *d = (f16)o[0];
         }
       }
     }
@@ -297,16 +365,16 @@ __global__ __launch_bounds__(1024) void ea_ln_join_kernel(const float* part, flo
 bool ln_vec(int C, const void* a, const void* b, const void* c, const void* d, const void* e, const void* f) {
   return (C & 7) == 0 && ((((uintptr_t)a) | ((uintptr_t)b) | ((uintptr_t)c) | ((uintptr_t)d) | ((uintptr_t)e) | ((uintptr_t)f)) & 15) == 0;
 }
-// lanes per row: the fewest that hold a row in at most 5 (8 lanes: 6) vectors of 8 columns; scalars always take the wave
-int ln_lanes(int C, bool vec) { return !vec ? 64 : C <= 384 ? 8 : C <= 640 ? 16 : C <= 1280 ? 32 : 64; }
+// lanes per row; scalars always take the wave
+int ln_lanes(int C, bool vec) { return !vec ? 64 : C <= 384 ? 16 : C <= 768 ? 32 : 64; }
 
 template <int XK, bool OUT8>
 int ln_train_launch(const LnTrainParams& p, bool vec, void* stream) {
   void (*k)(LnTrainParams);
   const int lpr = ln_lanes(p.C, vec);
   if (vec) {
-    k = lpr == 8 ? ea_ln_train_kernel<XK, 8, 8, 6, OUT8> : lpr == 16 ? ea_ln_train_kernel<XK, 8, 16, 5, OUT8>
-      : lpr == 32 ? ea_ln_train_kernel<XK, 8, 32, 5, OUT8> : p.C <= 2560 ? ea_ln_train_kernel<XK, 8, 64, 5, OUT8>
+    k = lpr == 16 ? ea_ln_train_kernel<XK, 8, 16, 3, OUT8> : lpr == 32 ? ea_ln_train_kernel<XK, 8, 32, 3, OUT8>
+      : p.C <= 1536 ? ea_ln_train_kernel<XK, 8, 64, 3, OUT8> : p.C <= 2560 ? ea_ln_train_kernel<XK, 8, 64, 5, OUT8>
       : ea_ln_train_kernel<XK, 8, 64, 8, OUT8>;
   } else {
     k = p.C <= 512 ? ea_ln_train_kernel<XK, 1, 64, 8, OUT8> : p.C <= 1536 ? ea_ln_train_kernel<XK, 1, 64, 24, OUT8>
@@ -317,24 +385,26 @@ int ln_train_launch(const LnTrainParams& p, bool vec, void* stream) {
   return ea_launch_status();
 }
 
-constexpr int LN_MAX_WG = 512;
+// Workgroups of the backward pass: as many as are resident (two per CU up to 1536 columns, one above), each walking the rows.  us for
+// 256 / 512 / 1024: 32768 x 320 23.1 / 22.8 / 28.3, 32768 x 1280 47.8 / 45.1 / 49.2, 4096 x 4096 34.9 / 43.1 / 60.9.
 int ln_bwd_grid(int M, int C) {            // the same for both paths of a width: the workspace does not depend on alignment
   const int rows = 4 * (64 / ln_lanes(C, (C & 7) == 0));
   const int g = (M + rows - 1) / rows;
-  return g < LN_MAX_WG ? g : LN_MAX_WG;
+  const int most = C > 1536 ? 256 : 512;
+  return g < most ? g : most;
 }
 
-template <int XK>
+template <int XK, bool F32>
 int ln_bwd_launch(const LnBwdParams& p, bool vec, int grid, void* stream) {
   void (*k)(LnBwdParams);
   const int lpr = ln_lanes(p.C, vec);
   if (vec) {
-    k = lpr == 8 ? ea_ln_bwd_kernel<XK, 8, 8, 6> : lpr == 16 ? ea_ln_bwd_kernel<XK, 8, 16, 5>
-      : lpr == 32 ? ea_ln_bwd_kernel<XK, 8, 32, 5> : p.C <= 2560 ? ea_ln_bwd_kernel<XK, 8, 64, 5>
-      : ea_ln_bwd_kernel<XK, 8, 64, 8>;
+    k = lpr == 16 ? ea_ln_bwd_kernel<XK, F32, 8, 16, 3> : lpr == 32 ? ea_ln_bwd_kernel<XK, F32, 8, 32, 3>
+      : p.C <= 1536 ? ea_ln_bwd_kernel<XK, F32, 8, 64, 3> : p.C <= 2560 ? ea_ln_bwd_kernel<XK, F32, 8, 64, 5>
+      : ea_ln_bwd_kernel<XK, F32, 8, 64, 8>;
   } else {
-    k = p.C <= 512 ? ea_ln_bwd_kernel<XK, 1, 64, 8> : p.C <= 1536 ? ea_ln_bwd_kernel<XK, 1, 64, 24>
-      : ea_ln_bwd_kernel<XK, 1, 64, 64>;
+    k = p.C <= 512 ? ea_ln_bwd_kernel<XK, F32, 1, 64, 8> : p.C <= 1536 ? ea_ln_bwd_kernel<XK, F32, 1, 64, 24>
+      : ea_ln_bwd_kernel<XK, F32, 1, 64, 64>;
   }
   const int smem = 4 * p.C * (int)sizeof(float);
   ea_allow_big_lds(k, smem);
@@ -363,7 +433,7 @@ extern "C" size_t ea_layernorm_bwd_workspace_bytes(int M, int C) {
 }
 
 extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const unsigned char* x_scale, const float* stats,
-                                const float* gamma, const void* residual, void* dx, int dx_f32, float* dgamma, float* dbeta, int M, int C,
+                                const float* gamma, const void* residual, void* dx, float* dgamma, float* dbeta, int M, int C,
                                 void* workspace, size_t ws_bytes, void* stream) {
   if (!dy || !x || !stats || !gamma || !dx || !dgamma || !dbeta || !workspace || (x_kind == XK_FP8 && !x_scale)) return EA_ERR_BAD_ARG;
   if (x_kind < XK_F16 || x_kind > XK_FP8) return EA_ERR_BAD_ARG;
@@ -371,14 +441,14 @@ extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const
   if (((uintptr_t)stats & 7) || ((uintptr_t)workspace & 3)) return EA_ERR_BAD_ARG;
   if (ws_bytes < ea_layernorm_bwd_workspace_bytes(M, C)) return EA_ERR_WORKSPACE;
   LnBwdParams p;
-  p.dy = (const f16*)dy; p.x = x; p.x_scale = x_scale; p.stats = stats; p.gamma = gamma; p.residual = residual; p.dx = dx; p.dx_f32 = dx_f32;
+  p.dy = (const f16*)dy; p.x = x; p.x_scale = x_scale; p.stats = stats; p.gamma = gamma; p.residual = residual; p.dx = dx;
   p.part = (float*)workspace; p.M = M; p.C = C;
   p.xpitch = x_kind == XK_FP8 ? ea_fp8_blocks(C) * EA_FP8_BLOCK : C;
   p.xspitch = ea_fp8_scale_pitch(M);
   const bool vec = ln_vec(C, dy, x, gamma, residual, dx, nullptr);
   const int grid = ln_bwd_grid(M, C);
-  const int st = x_kind == XK_F16 ? ln_bwd_launch<XK_F16>(p, vec, grid, stream) : x_kind == XK_F32 ? ln_bwd_launch<XK_F32>(p, vec, grid, stream)
-                                  : ln_bwd_launch<XK_FP8>(p, vec, grid, stream);
+  const int st = x_kind == XK_F16 ? ln_bwd_launch<XK_F16, false>(p, vec, grid, stream)
+               : x_kind == XK_F32 ? ln_bwd_launch<XK_F32, true>(p, vec, grid, stream) : ln_bwd_launch<XK_FP8, false>(p, vec, grid, stream);
   if (st != EA_OK) return st;
   auto k = ea_ln_join_kernel;
   EA_LAUNCH(k, dim3((2 * C + 31) / 32), dim3(1024), 32 * 33 * sizeof(float), stream, (const float*)workspace, dgamma, dbeta, grid, C);

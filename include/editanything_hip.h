@@ -419,13 +419,13 @@ int ea_activation_fp8(const void* z, int act, void* h, void* hq, unsigned char* 
                       void* stream);
 int ea_activation_fp8_bwd(const void* dh, const void* zq, const unsigned char* zscale, int act, void* dz, long long M, int H, void* stream);
 /* LayerNorm for training, C <= 4096.  Forward: y fp16 or q / scale in 8 bits (exactly one of y, q), stats fp32 [M][2] = (mean,
- * 1 / sigma).  Backward: x_kind 0 fp16, 1 fp32, 2 8-bit (x_scale); residual (NULL: none) is added to dx and has its type (fp16, or
- * fp32 where dx_f32); dgamma, dbeta fp32 [C], reduced in a fixed order. */
+ * 1 / sigma).  Backward: x_kind 0 fp16, 1 fp32, 2 8-bit (x_scale); residual (NULL: none) is added to dx; both are fp32 for an
+ * fp32 x and fp16 otherwise; dgamma, dbeta fp32 [C], reduced in a fixed order. */
 int ea_layernorm_train(const void* x, int in_f32, const float* gamma, const float* beta, float eps, void* y, void* q, unsigned char* scale,
                        float* stats, int M, int C, void* stream);
 size_t ea_layernorm_bwd_workspace_bytes(int M, int C);
 int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const unsigned char* x_scale, const float* stats, const float* gamma,
-                     const void* residual, void* dx, int dx_f32, float* dgamma, float* dbeta, int M, int C, void* workspace,
+                     const void* residual, void* dx, float* dgamma, float* dbeta, int M, int C, void* workspace,
                      size_t ws_bytes, void* stream);
 /* out = residual + scale * act(A W^T + bias): A 8-bit rows [M][Kp], W an 8-bit weight [N][Kp].  Of the epilogue: bias (per column), act
  * (none, SiLU, GELU), scale, residual or residual32, out / out_f32, ldc, ldr; anything else is EA_ERR_UNSUPPORTED. */

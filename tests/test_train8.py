@@ -339,7 +339,7 @@ def test_layernorm_backward(kb, M, C, kind, res):
     st = np.stack([mu, r], 1).astype(np.float32)
     dx, dg, db = kb.up(np.full((M + 1, C), 7, out)), kb.zeros((C,), np.float32), kb.zeros((C,), np.float32)
     ws = kb.zeros((kb.lib.ea_layernorm_bwd_workspace_bytes(M, C) // 4,), np.float32)
-    args = (ptr(dy), ptr(x), kind, ptr(xs), ptr(st), ptr(gamma), ptr(residual), ptr(dx), int(kind == 1), ptr(dg), ptr(db), M, C, ptr(ws))
+    args = (ptr(dy), ptr(x), kind, ptr(xs), ptr(st), ptr(gamma), ptr(residual), ptr(dx), ptr(dg), ptr(db), M, C, ptr(ws))
     assert kb.lib.ea_layernorm_bwd(*args, ws.nbytes - 1 if kb.name == "emu" else ws.numel() * 4 - 1, kb.stream) == -4
     assert kb.lib.ea_layernorm_bwd(*args, ws.nbytes if kb.name == "emu" else ws.numel() * 4, kb.stream) == 0
     mu, r = st.astype(np.float64).T
@@ -553,10 +553,10 @@ def test_the_c_entries_refuse(emu_lib):
     assert lib.ea_layernorm_train(p, 0, p, p, 1e-5, None, None, None, p, 1, 8, None) == -2
     assert lib.ea_layernorm_train(p, 0, p, p, 1e-5, o, None, None, p, 1, 4097, None) == -1
     assert lib.ea_layernorm_train(p, 0, p, p, 1e-5, o, None, None, p + 4, 1, 8, None) == -2
-    assert lib.ea_layernorm_bwd(p, p, 3, None, p, p, None, o, 0, o, o, 1, 8, p, 1 << 20, None) == -2
-    assert lib.ea_layernorm_bwd(p, p, 2, None, p, p, None, o, 0, o, o, 1, 8, p, 1 << 20, None) == -2
-    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, 0, o, o, 1, 5000, p, 1 << 20, None) == -1
-    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, 0, o, o, 1, 8, p, 0, None) == -4
+    assert lib.ea_layernorm_bwd(p, p, 3, None, p, p, None, o, o, o, 1, 8, p, 1 << 20, None) == -2
+    assert lib.ea_layernorm_bwd(p, p, 2, None, p, p, None, o, o, o, 1, 8, p, 1 << 20, None) == -2
+    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, o, o, 1, 5000, p, 1 << 20, None) == -1
+    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, o, o, 1, 8, p, 0, None) == -4
     assert lib.ea_layernorm_bwd_workspace_bytes(0, 8) == 0 and lib.ea_layernorm_bwd_workspace_bytes(1, 4097) == 0
     e = epilogue(a)
     g = lambda **kw: lib.ea_gemm_fp8(kw.get("a", p), kw.get("sa", p), p, p, kw.get("M", 16), kw.get("N", 16), kw.get("K", 128),  # noqa: E731

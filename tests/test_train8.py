@@ -619,3 +619,210 @@ def test_the_public_functions_refuse():
               lambda: ops.activation_fp8_backward(f16, t, ops.ACT_SILU), lambda: ops.gemm_fp8(t, w), lambda: ops.gemm_fp8_wgrad(f16, t)):
         with pytest.raises(RuntimeError, match="MI355X"):      # no CPU path
             f()
+
+
+# ------------------------------------------------------------------------------------------- the public functions, on the GPU
+def block_inputs(seed, shape, hidden, dtype=torch.float16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    C = shape[-1]
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    return dict(x=r(*shape).to(dtype), gamma=1 + 0.2 * r(C), beta=0.1 * r(C), w1=r(hidden, C) * C ** -0.5, b1=0.1 * r(hidden),
+                w2=r(C, hidden) * hidden ** -0.5, b2=0.1 * r(C), dout=(0.02 * r(*shape)).half())
+
+
+def block_weights(s):
+    return dict(q1=ops.quantize_fp8_weight(s["w1"]), q2=ops.quantize_fp8_weight(s["w2"]), q1t=ops.quantize_fp8_weight(s["w1"].t().contiguous()),
+                q2t=ops.quantize_fp8_weight(s["w2"].t().contiguous()))
+
+
+def block(s, w):
+    """x + Linear(GELU(Linear(LayerNorm(x)))), forward and backward, what is kept for the backward pass in 8 bits."""
+    y8, stats = ops.layernorm_train(s["x"], s["gamma"], s["beta"], fp8=True)
+    z = ops.gemm_fp8(y8, w["q1"], bias=s["b1"])
+    h8, z8 = ops.activation_fp8(z, ops.ACT_GELU, fp8=True)
+    out = ops.gemm_fp8(h8, w["q2"], bias=s["b2"], residual=s["x"])
+    d8 = ops.quantize_fp8(s["dout"])
+    dh = ops.gemm_fp8(d8, w["q2t"])
+    dw2, db2 = ops.gemm_fp8_wgrad(s["dout"], h8)
+    dz = ops.activation_fp8_backward(dh, z8, ops.ACT_GELU)
+    dy = ops.gemm_fp8(ops.quantize_fp8(dz), w["q1t"])
+    dw1, db1 = ops.gemm_fp8_wgrad(dz, y8)
+    dx, dgamma, dbeta = ops.layernorm_backward(dy, s["x"], stats, s["gamma"], residual=s["dout"])
+    return dict(y=y8.q, ys=y8.scale[:, :y8.rows], stats=stats, z=z, h=h8.q, hs=h8.scale[:, :h8.rows], zq=z8.q, out=out, dh=dh, dz=dz, dy=dy, dw1=dw1,
+                db1=db1, dw2=dw2, db2=db2, dx=dx, dgamma=dgamma, dbeta=dbeta)
+
+
+def same_bits(a, b):
+    return all(torch.equal(a[k].view(torch.uint8) if a[k].dtype == torch.float8_e4m3fn else a[k],
+                           b[k].view(torch.uint8) if b[k].dtype == torch.float8_e4m3fn else b[k]) for k in a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,hidden", [((2, 77, 320), 1280), ((3, 5, 136), 264), ((1, 1, 640), 640)])
+def test_block_step_by_step(shape, hidden):
+    """Every step of a whole block against the same step in 64 bits on the operands that it was really given."""
+    s = block_inputs(1, shape, hidden)
+    w = block_weights(s)
+    M, C = shape[0] * shape[1], shape[2]
+    d = lambda t: t.double().reshape(M, -1)  # noqa: E731
+    v = lambda q, sc, c: ops.Fp8Tensor(q, torch.nn.functional.pad(sc, (0, -M % 16)).contiguous(), c).dequantize(torch.float32).double()  # noqa: E731
+    r = block(s, w)
+    assert tuple(r["out"].shape) == shape and tuple(r["z"].shape) == shape[:2] + (hidden,) and tuple(r["dx"].shape) == shape
+    y, h = v(r["y"], r["ys"], C), v(r["h"], r["hs"], hidden)
+    W1, W2 = (w[k].dequantize(torch.float32).double() for k in ("q1", "q2"))
+    near = lambda got, ref, mag, n: ((d(got) - ref).abs() <= (2 * (n + 2) * U32 + UNIT) * mag + U16 * ref.abs() + TINY16 + 8 * U32 * ref.abs()).all()  # noqa: E731
+    assert near(r["z"], y @ W1.t().contiguous() + s["b1"].double(), y.abs() @ W1.abs().t().contiguous(), C)
+    res = d(s["x"])
+    assert near(r["out"], h @ W2.t().contiguous() + s["b2"].double() + res, h.abs() @ W2.abs().t().contiguous() + res.abs(), hidden)
+    dq = ops.quantize_fp8(s["dout"]).dequantize(torch.float32).double().reshape(M, C)
+    assert near(r["dh"], dq @ W2, dq.abs() @ W2.abs(), C)
+    zq = ops.quantize_fp8(r["z"]).dequantize(torch.float32).double().reshape(M, hidden)
+    slope = 0.5 * torch.erfc(-zq / math.sqrt(2)) + zq * torch.exp(-zq * zq / 2) / math.sqrt(2 * math.pi)
+    ref = d(r["dh"]) * slope
+    assert ((d(r["dz"]) - ref).abs() <= U16 * ref.abs() + TINY16 + ACT_ABS * d(r["dh"]).abs() * zq.abs().clamp_min(1) + 8 * U32 * ref.abs()).all()
+    eq = ops.quantize_fp8(r["dz"]).dequantize(torch.float32).double().reshape(M, hidden)
+    assert near(r["dy"], eq @ W1, eq.abs() @ W1.abs(), hidden)
+    for dw, db, dd, xx in ((r["dw1"], r["db1"], d(r["dz"]), y), (r["dw2"], r["db2"], d(s["dout"]), h)):
+        tol = 2 * (M + 2) * U32 * (dd.abs().t().contiguous() @ xx.abs()) + 2.0 ** -24 * dd.abs().sum(0)[:, None] + 1e-30
+        assert ((dw.double() - dd.t().contiguous() @ xx).abs() <= tol).all()
+        assert ((db.double() - dd.sum(0)).abs() <= 2 * (M + 2) * U32 * dd.abs().sum(0)).all()
+    mu, rs = r["stats"][:, :1].double(), r["stats"][:, 1:].double()
+    n, g = (d(s["x"]) - mu) * rs, d(r["dy"]) * s["gamma"].double()
+    s1, s2 = g.mean(1, keepdim=True), (g * n).mean(1, keepdim=True)
+    ref = rs * (g - s1 - n * s2) + d(s["dout"])
+    mag = rs * (g.abs() + g.abs().mean(1, keepdim=True) + n.abs() * (g * n).abs().mean(1, keepdim=True)) + d(s["dout"]).abs()
+    assert ((d(r["dx"]) - ref).abs() <= U16 * ref.abs() + TINY16 + (2 * C + 16) * U32 * mag).all()
+    for got, terms in ((r["dgamma"], d(r["dy"]) * n), (r["dbeta"], d(r["dy"]))):
+        assert ((got.double() - terms.sum(0)).abs() <= (M + 16) * U32 * terms.abs().sum(0) + 1e-30).all()
+
+
+@pytest.mark.gpu
+def test_a_block_repeats_bit_for_bit_on_any_stream():
+    s = block_inputs(2, (2, 333, 640), 2560)
+    w = block_weights(s)
+    ref = block(s, w)
+    assert same_bits(ref, block(s, w))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        t = {k: v.clone() for k, v in s.items()}
+        got = block(t, block_weights(t))
+    # ... beside matrix products on the main stream
+    a = torch.randn(4096, 4096, device="cuda", dtype=torch.float16)
+    for _ in range(20):
+        a = (a @ a).clamp_(-1, 1)
+    for _ in range(4):
+        with torch.cuda.stream(side):
+            got2 = block(t, block_weights(t))
+        a = (a @ a).clamp_(-1, 1)
+    torch.cuda.synchronize()
+    assert same_bits(ref, got) and same_bits(ref, got2)
+
+
+@pytest.mark.gpu
+def test_a_captured_block_replays_with_new_inputs():
+    """Two graphs of two blocks, replayed on two streams at once, several times, with eager work in between: always the eager result."""
+    cases = []
+    for seed, shape, hidden in ((3, (2, 100, 320), 1280), (4, (1, 640, 648), 1296)):
+        s = block_inputs(seed, shape, hidden)
+        w = block_weights(s)
+        block(s, w)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = block(s, w)
+        cases.append((s, w, g, out, torch.cuda.Stream()))
+    for k in range(4):
+        refs = []
+        for s, w, g, out, st in cases:
+            for name, t in block_inputs(10 + k, s["x"].shape, s["w1"].shape[0]).items():
+                if name in ("x", "dout"):
+                    s[name].copy_(t)
+            refs.append({n: t.clone() for n, t in block(s, w).items()})
+        torch.cuda.synchronize()
+        for s, w, g, out, st in cases:
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for ref, (s, w, g, out, st) in zip(refs, cases):
+            assert same_bits(ref, out), k
+
+
+@pytest.mark.gpu
+def test_empty_and_unaligned_inputs():
+    e16, one = torch.empty(0, 5, 320, device="cuda", dtype=torch.float16), torch.ones(320, device="cuda")
+    q = ops.quantize_fp8(e16)
+    assert tuple(q.shape) == (0, 5, 320) and tuple(q.dequantize().shape) == (0, 5, 320)
+    y, st = ops.layernorm_train(e16, one, one)
+    dx, dg, db = ops.layernorm_backward(e16, e16, st, one)
+    assert y.numel() == dx.numel() == st.numel() == 0 and not dg.any() and not db.any() and dg.shape == (320,)
+    h, z = ops.activation_fp8(e16, ops.ACT_GEGLU)
+    assert tuple(h.shape) == (0, 5, 160) and tuple(ops.activation_fp8_backward(h, z, ops.ACT_GEGLU).shape) == (0, 5, 320)
+    w = ops.quantize_fp8_weight(torch.randn(24, 320, device="cuda"))
+    assert tuple(ops.gemm_fp8(q, w).shape) == (0, 5, 24)
+    dw, b = ops.gemm_fp8_wgrad(torch.empty(0, 5, 24, device="cuda", dtype=torch.float16), q)
+    assert tuple(dw.shape) == (24, 320) and not dw.any() and not b.any()
+    # contiguous, but one element off every alignment: the same rules of arithmetic, another code path
+    g = torch.Generator(device="cuda").manual_seed(5)
+    odd = lambda *s: torch.randn(math.prod(s) + 1, generator=g, device="cuda").half()[1:].view(*s)  # noqa: E731
+    x, dy, res = odd(70, 320), odd(70, 320), odd(70, 320)
+    qa, qb = ops.quantize_fp8(x), ops.quantize_fp8(x.clone())
+    assert torch.equal(qa.q.view(torch.uint8), qb.q.view(torch.uint8)) and torch.equal(qa.scale[:, :70], qb.scale[:, :70])
+    for act in (ops.ACT_SILU, ops.ACT_GEGLU):
+        a, sa = ops.activation_fp8(x, act)
+        b, sb = ops.activation_fp8(x.clone(), act)
+        dh = odd(*a.shape)
+        assert torch.equal(sa.q.view(torch.uint8), sb.q.view(torch.uint8))
+        # two compilations of one formula: each within half a step of fp16 and ACT_ABS times its factors of the exact value
+        for u, v in ((a, b), (ops.activation_fp8_backward(dh, sa, act), ops.activation_fp8_backward(dh.clone(), sb, act))):
+            slack = 2 * TINY16 + 2 * ACT_ABS * float(x.abs().max().clamp_min(1) * dh.abs().max().clamp_min(1))
+            assert ((u.double() - v.double()).abs() <= 2 * U16 * 1.001 * v.double().abs() + slack).all()
+    close = lambda a, b, tol: (a.double() - b.double()).abs().max() <= tol * b.double().abs().max()  # noqa: E731
+    ga = torch.randn(321, generator=g, device="cuda")[1:]
+    (y1, s1), (y2, s2) = ops.layernorm_train(x, ga, ga), ops.layernorm_train(x.clone(), ga.clone(), ga.clone())
+    assert close(y1, y2, 2 * U16) and close(s1, s2, 64 * U32)
+    r1, r2 = ops.layernorm_backward(dy, x, s2, ga, res), ops.layernorm_backward(dy.clone(), x.clone(), s2, ga.clone(), res.clone())
+    assert close(r1[0], r2[0], 2 * U16) and close(r1[1], r2[1], 1024 * U32) and close(r1[2], r2[2], 1024 * U32)
+    w = ops.quantize_fp8_weight(torch.randn(24, 320, generator=g, device="cuda"))
+    rs, o = odd(70, 24), odd(70, 24)
+    assert torch.equal(ops.gemm_fp8(qa, w, residual=rs, out=o), ops.gemm_fp8(qa, w, residual=rs.clone()))
+    (a1, b1), (a2, b2) = ops.gemm_fp8_wgrad(rs, qa), ops.gemm_fp8_wgrad(rs.clone(), qa)
+    assert close(a1, a2, 1024 * U32) and close(b1, b2, 1024 * U32)
+
+
+@pytest.mark.gpu
+def test_offsets_behind_32_bits():
+    """More than 2^31 bytes of codes and 2^32 bytes of fp16: the first and the last rows, and sums over all of them."""
+    M, K, N = 1_100_001, 2048, 16
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(M, K, generator=g, device="cuda", dtype=torch.float16)
+    q = ops.quantize_fp8(x)
+    pick = torch.tensor([0, 1, 1_048_575, 1_048_576, M - 17, M - 1], device="cuda")
+    few = ops.quantize_fp8(x[pick].contiguous())
+    assert torch.equal(q.q.view(torch.uint8)[pick], few.q.view(torch.uint8)) and torch.equal(q.scale[:, pick], few.scale[:, :6])
+    assert torch.equal(q.dequantize()[pick], few.dequantize())
+    w = ops.quantize_fp8_weight(torch.randn(N, K, generator=g, device="cuda"))
+    assert torch.equal(ops.gemm_fp8(q, w)[pick], ops.gemm_fp8(few, w))
+    dy = (0.02 * torch.randn(M, N, generator=g, device="cuda")).half()
+    dw, db = ops.gemm_fp8_wgrad(dy, q)
+    ref, mag, step = torch.zeros(N, K, device="cuda", dtype=torch.float64), torch.zeros(N, K, device="cuda", dtype=torch.float64), 110_000
+    for a in range(0, M, step):
+        d, v = dy[a:a + step].double(), ops.Fp8Tensor(q.q[a:a + step], torch.nn.functional.pad(q.scale[:, a:min(a + step, M)],
+                                                      (0, -min(step, M - a) % 16)).contiguous(), K).dequantize(torch.float32).double()
+        ref += d.t().contiguous() @ v
+        mag += d.abs().t().contiguous() @ v.abs()
+    # n independent terms of size s: the partial sums grow like sqrt(k) s, each addition is off by at most 2 u32 of its partial sum, with
+    # either sign: together 2 u32 s sqrt(1 + 2 + ... + n) = 1.4 u32 n s, under 2 u32 of the sum of magnitudes; 16 times that is allowed
+    assert ((dw.double() - ref).abs() <= 32 * U32 * mag).all()
+    assert ((db.double() - dy.double().sum(0)).abs() <= 32 * U32 * dy.double().abs().sum(0)).all()
+    h, z = ops.activation_fp8(x, ops.ACT_GELU)
+    h2, z2 = ops.activation_fp8(x[pick].contiguous(), ops.ACT_GELU)
+    assert torch.equal(h[pick], h2) and torch.equal(z.q.view(torch.uint8)[pick], z2.q.view(torch.uint8))
+    del h, z
+    one = torch.ones(K, device="cuda")
+    y, st = ops.layernorm_train(x, one, one)
+    y2, st2 = ops.layernorm_train(x[pick].contiguous(), one, one)
+    assert torch.equal(y[pick], y2) and torch.equal(st[pick], st2)
+    dx, dg, db = ops.layernorm_backward(y, x, st, one)
+    assert torch.equal(dx[pick], ops.layernorm_backward(y2, x[pick].contiguous(), st2, one)[0])
+    assert ((db.double() - y.sum(0, dtype=torch.float64)).abs() <= 32 * U32 * y.abs().sum(0, dtype=torch.float64)).all()

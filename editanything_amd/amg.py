@@ -335,7 +335,7 @@ class SamPromptDecoder:
             cur.wait_stream(side)
             try:
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, capture_error_mode="thread_local"):
+                with ops.graph_capture(g, capture_error_mode="thread_local"):
                     out = self.predict_masks(tok_s, emb_hw, sp_s, multimask_output)
             except Exception as exc:                                           # noqa: BLE001 -- any capture failure: eager from now on
                 import warnings

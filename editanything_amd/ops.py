@@ -6,6 +6,7 @@ libeditanything_hip.so on `torch.cuda.current_stream()`.  Activations are NHWC f
 There is no eager/CPU fallback: tensors must live on the MI355X.
 """
 import ctypes as C
+import gc
 import math
 import threading
 
@@ -104,6 +105,45 @@ class aux_workspace:
 
     def __exit__(self, *exc):
         _tls.aux = self._prev
+
+
+class graph_capture:
+    """with ops.graph_capture(graph, ...): torch.cuda.graph with Python's cyclic garbage collection held off until the capture has ended.
+    A collection that happens to start inside a capture and finds a dead CUDAGraph (an object of a reference cycle: a dropped
+    pipeline, a test's fixture) runs its destructor, which synchronises the device on ROCm; that is an error while a stream is being captured,
+    and an error in a destructor ends the process.  Captures of several threads may overlap: the last one out lets collection go on."""
+    _lock = threading.Lock()
+    _held, _was_on = 0, False
+
+    def __init__(self, graph, **kw):
+        self._ctx = torch.cuda.graph(graph, **kw)
+
+    def __enter__(self):
+        cls = graph_capture
+        with cls._lock:
+            if cls._held == 0:
+                cls._was_on = gc.isenabled()
+                gc.disable()
+            cls._held += 1
+        try:
+            return self._ctx.__enter__()
+        except BaseException:
+            self._release()
+            raise
+
+    def __exit__(self, *exc):
+        try:
+            return self._ctx.__exit__(*exc)
+        finally:
+            self._release()
+
+    @staticmethod
+    def _release():
+        cls = graph_capture
+        with cls._lock:
+            cls._held -= 1
+            if cls._held == 0 and cls._was_on:
+                gc.enable()
 
 
 class Pair:

@@ -764,7 +764,7 @@ class StableDiffusionControlNetInpaintPipeline:
 
         def instantiate():
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
+            with ops.graph_capture(g):
                 step()
             restore()
             return g

@@ -32,6 +32,14 @@ def pytest_collection_modifyitems(config, items):
         items[:] = keep
 
 
+def pytest_runtest_teardown(item, nextitem):
+    """Dead cycles of a module's fixtures (captured graphs among them) go between modules, not inside a later test's own graph capture,
+    where the destructor of a graph ends the process (ops.graph_capture)."""
+    if nextitem is None or getattr(nextitem, "module", None) is not getattr(item, "module", None):
+        import gc
+        gc.collect()
+
+
 @pytest.fixture(scope="session")
 def emu_lib():
     """Host emulation build of the HIP kernels (tests/emu) bound through the same ctypes prototypes."""

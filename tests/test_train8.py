@@ -621,6 +621,48 @@ def test_the_public_functions_refuse():
             f()
 
 
+# --------------------------------------------------------------------------------------------------------- capturing, on the CPU
+def test_no_garbage_collection_inside_a_capture(monkeypatch):
+    """A dead cycle is not collected while any thread captures, and collection is as it was afterwards, also behind errors."""
+    import gc
+    import threading
+
+    class Fake:
+        def __init__(self, graph, fail=False, **kw):
+            self.fail = fail
+
+        def __enter__(self):
+            if self.fail:
+                raise RuntimeError("no capture")
+
+        def __exit__(self, *exc):
+            return None
+    monkeypatch.setattr(torch.cuda, "graph", Fake)
+    assert gc.isenabled()
+    with ops.graph_capture(None, capture_error_mode="thread_local"):
+        assert not gc.isenabled()
+        t = threading.Thread(target=lambda: ops.graph_capture(None).__enter__())      # a capture that is still open on another thread
+        t.start()
+        t.join()
+    assert not gc.isenabled()
+    ops.graph_capture(None).__exit__(None, None, None)
+    assert gc.isenabled()
+    with pytest.raises(RuntimeError):
+        with ops.graph_capture(None, fail=True):
+            pass
+    with pytest.raises(KeyError):
+        with ops.graph_capture(None):
+            raise KeyError
+    assert gc.isenabled()
+    gc.disable()
+    try:
+        with ops.graph_capture(None):
+            pass
+        assert not gc.isenabled()                               # it was off before
+    finally:
+        gc.enable()
+
+
 # ------------------------------------------------------------------------------------------- the public functions, on the GPU
 def block_inputs(seed, shape, hidden, dtype=torch.float16):
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -729,7 +771,7 @@ def test_a_captured_block_replays_with_new_inputs():
         block(s, w)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with ops.graph_capture(g):
             out = block(s, w)
         cases.append((s, w, g, out, torch.cuda.Stream()))
     for k in range(4):

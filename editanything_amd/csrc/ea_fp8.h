@@ -19,6 +19,14 @@
 #define EA_FP8_E_MAX 120
 #define EA_INF_BITS 0x7f800000u
 
+// 16 bytes at any element's alignment (global memory takes unaligned vector accesses; a row of odd length starts anywhere)
+typedef f16x8 f16x8_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+__device__ __forceinline__ f16x8 ea_ld8u(const f16* p) { return *reinterpret_cast<const f16x8_any*>(p); }
+__device__ __forceinline__ void ea_st8u(f16* p, f16x8 v) { *reinterpret_cast<f16x8_any*>(p) = v; }
+__device__ __forceinline__ f32x4 ea_ld4u(const float* p) { return *reinterpret_cast<const f32x4_any*>(p); }
+__device__ __forceinline__ void ea_st4u(float* p, f32x4 v) { *reinterpret_cast<f32x4_any*>(p) = v; }
+
 __device__ __forceinline__ unsigned ea_f2u(float v) { return __builtin_bit_cast(unsigned, v); }
 __device__ __forceinline__ float ea_u2f(unsigned v) { return __builtin_bit_cast(float, v); }
 // |v| where it enters a block's maximum: NaN and infinity count as 0

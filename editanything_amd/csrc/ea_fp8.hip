@@ -34,7 +34,18 @@ __device__ __forceinline__ void q_load8(const void* x, long long row, int cols, 
     if (c >= cols)
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-  } else {
+  } else if (c + 8 <= cols) {                                 // a row that starts anywhere
+    if constexpr (F32) {
+      const float* p = (const float*)x + row * cols + c;
+      const f32x4 a = ea_ld4u(p), b = ea_ld4u(p + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    } else {
+      const f16x8 h = ea_ld8u((const f16*)x + row * cols + c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+    }
+  } else {                                                    // its end
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       v[j] = c + j < cols ? (F32 ? ((const float*)x)[row * cols + c + j] : (float)((const f16*)x)[row * cols + c + j]) : 0.0f;
@@ -50,6 +61,7 @@ __device__ __forceinline__ f16x8 q_load8h(const f16* x, long long row, int cols,
     return h;
   } else {
     f16x8 h;
+    if (c + 8 <= cols) return ea_ld8u(x + row * cols + c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) h[j] = c + j < cols ? x[row * cols + c + j] : (f16)0.0f;
     return h;
@@ -140,6 +152,10 @@ __device__ __forceinline__ void h_load8(const f16* p, int c, int cols, float* v)
     const f16x8 h = ea_ld8(p + (c < cols ? c : 0));
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+  } else if (c + 8 <= cols) {
+    const f16x8 h = ea_ld8u(p + c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? (float)p[c + j] : 0.0f;
@@ -152,6 +168,11 @@ __device__ __forceinline__ void h_store8(f16* p, int c, int cols, const float* v
 #pragma unroll
     for (int j = 0; j < 8; ++j) h[j] = (f16)v[j];
     if (c < cols) ea_st8(p + c, h);
+  } else if (c + 8 <= cols) {
+    f16x8 h;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = (f16)v[j];
+    ea_st8u(p + c, h);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -178,6 +199,9 @@ __global__ __launch_bounds__(256) void ea_dequant_kernel(const uint8_t* q, const
       if (VEC && c < cols) {
         *reinterpret_cast<f32x4*>(o + c) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4*>(o + c + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      } else if (!VEC && c + 8 <= cols) {
+        ea_st4u(o + c, f32x4{v[0], v[1], v[2], v[3]});
+        ea_st4u(o + c + 4, f32x4{v[4], v[5], v[6], v[7]});
       } else if (!VEC) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)

@@ -95,6 +95,8 @@ __global__ __launch_bounds__(256) void ea_fp8_wgrad_kernel(WgradParams p) {
       if (p.vec) {
         dr[i] = ea_ld8(d + (n < p.N ? n : 0));
         if (!ok || n >= p.N) dr[i] = ea_zero8();
+      } else if (ok && n + 8 <= p.N) {
+        dr[i] = ea_ld8u(d + n);            // (rows that start anywhere)
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) dr[i][j] = ok && n + j < p.N ? d[n + j] : (f16)0.0f;

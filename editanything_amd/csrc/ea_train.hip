@@ -23,159 +23,38 @@ namespace {
 
 enum { XK_F16 = 0, XK_F32 = 1, XK_FP8 = 2 };
 
-// VEC consecutive values of one row (VEC = 8: 16-byte loads, C a multiple of 8; VEC = 1: any C)
-template <int XK, int VEC>
-__device__ __forceinline__ void ld_row(const void* x, const uint8_t* scale, long long row, int pitch, long long spitch, int c, float* v) {
-  if constexpr (XK == XK_F16) {
-    const f16* p = (const f16*)x + row * pitch + c;
-    if constexpr (VEC == 8) {
-      const f16x8 h = ea_ld8(p);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
-    } else v[0] = (float)*p;
-  } else if constexpr (XK == XK_F32) {
-    const float* p = (const float*)x + row * pitch + c;
-    if constexpr (VEC == 8) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
-    } else v[0] = *p;
-  } else {
-    const uint8_t* p = (const uint8_t*)x + row * pitch + c;
-    const float s = ea_fp8_scale(scale[(long long)(c >> 7) * spitch + row]);
-    if constexpr (VEC == 8) {
-      const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-      ea_fp8_unpack4(w[0], v);
-      ea_fp8_unpack4(w[1], v + 4);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= s;
-    } else {
-      float t[4];
-      ea_fp8_unpack4(*p, t);
-      v[0] = t[0] * s;
-    }
-  }
-}
-
-template <int VEC>
-__device__ __forceinline__ void ld_f32(const float* p, float* v) {
-  if constexpr (VEC == 8) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
-  } else v[0] = *p;
-}
-
-// ------------------------------------------------------------------------------------------------------------ forward
-struct LnTrainParams {
-  const void* x; const float* gamma; const float* beta;
-  f16* y;                              // fp16 output, or NULL
-  uint8_t* q; uint8_t* scale;          // 8-bit output
-  float* stats;                        // [M][2]: mean, 1 / sigma
-  int M, C, Kp; long long Rp;
-  float eps;
-};
-
-template <int XK, int VEC, int LPR, int NV, bool OUT8>
-__global__ __launch_bounds__(256) void ea_ln_train_kernel(LnTrainParams p) {
-  constexpr int RPW = 64 / LPR;
-  const int lane = threadIdx.x & 63, sub = lane / LPR, l = lane % LPR;
-  const int row = (blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW + sub;
-  const int r = row < p.M ? row : p.M - 1;
-  float x[NV][VEC];
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (l + LPR * i) * VEC;
-    if (c < p.C) ld_row<XK, VEC>(p.x, nullptr, r, p.C, 0, c, x[i]);
-    else
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) x[i][j] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) s += x[i][j];
-  }
-  const float mean = ea_group_sum<LPR>(s) / (float)p.C;
-  float q = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (l + LPR * i) * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float d = c < p.C ? x[i][j] - mean : 0.0f;
-      q += d * d;
-    }
-  }
-  const float rstd = 1.0f / sqrtf(ea_group_sum<LPR>(q) / (float)p.C + p.eps);
-  if (row < p.M && l == 0) *reinterpret_cast<f32x2*>(p.stats + 2ll * row) = f32x2{mean, rstd};
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (l + LPR * i) * VEC;
-    if (c < p.C) {
-      float ga[VEC], be[VEC];
-      ld_f32<VEC>(p.gamma + c, ga);
-      ld_f32<VEC>(p.beta + c, be);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) x[i][j] = (x[i][j] - mean) * rstd * ga[j] + be[j];
-      if (!OUT8 && row < p.M) {
-        f16* o = p.y + (long long)row * p.C + c;
-        if constexpr (VEC == 8) {
-          f16x8 h;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) h[j] = (f16)x[i][j];
-          ea_st8(o, h);
-        } else *o = (f16)x[i][0];
-      }
-    }
-  }
-  if constexpr (OUT8) {
-    // a block of 128 columns: 16 lanes of one vector, or two scalars of the whole wave
-    if constexpr (VEC == 8) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (l + LPR * i) * 8;
-        int e;
-        const u32x2 w = ea_fp8_block<16>((const float*)x[i], e);
-        if (row < p.M && c < p.Kp) {
-          *reinterpret_cast<u32x2*>(p.q + (long long)row * p.Kp + c) = w;
-          if ((c & 127) == 0) p.scale[(long long)(c >> 7) * p.Rp + row] = (uint8_t)e;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NV; i += 2) {
-        const int e = ea_fp8_exp_byte(ea_group_max<64>(fmaxf(ea_finite_abs(x[i][0]), ea_finite_abs(x[i + 1][0]))));
-        const float inv = ea_fp8_inv_scale(e);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int c = l + 64 * (i + u);
-          if (row < p.M && c < p.Kp) {
-            p.q[(long long)row * p.Kp + c] = (uint8_t)ea_fp8_pack4(ea_fp8_prep(x[i + u][0], inv), 0.0f, 0.0f, 0.0f);
-            if ((c & 127) == 0) p.scale[(long long)(c >> 7) * p.Rp + row] = (uint8_t)e;
-          }
-        }
-      }
-    }
-  }
-}
-
-// ----------------------------------------------------------------------------------------------------------- backward
-struct LnBwdParams {
-  const f16* dy; const void* x; const uint8_t* x_scale; const float* stats; const float* gamma;
-  const void* residual; void* dx;
-  float* part;                         // [gridDim.x][2][C]
-  int M, C, xpitch; long long xspitch;
-};
-
-// VEC values as they lie in memory: loaded a row ahead, converted when they are used
-template <int XK, int VEC>
-struct Raw {
+// Eight consecutive values of a row of C, from column c < C on, as they lie in memory.  ANY: rows start anywhere and C is any number: 16
+// bytes at the type's own alignment, and the values one by one at the end of a row (what lies behind it is not read; it reads as 0).
+// Otherwise C is a multiple of 8 and everything is 16-byte aligned.  8-bit rows are padded to whole blocks: always aligned.
+template <int XK, bool ANY>
+struct Row8 {
   u32x4 a, b;                          // (fp32: both; fp16: a; codes: half of a and the scale byte in a[2])
-  __device__ __forceinline__ void load(const void* x, const uint8_t* scale, long long row, int pitch, long long spitch, int c) {
+  __device__ __forceinline__ void load(const void* x, const uint8_t* scale, long long row, int pitch, long long spitch, int c, int C) {
     if constexpr (XK == XK_F16) {
-      a = *reinterpret_cast<const u32x4*>((const f16*)x + row * pitch + c);
+      const f16* p = (const f16*)x + row * pitch + c;
+      if (!ANY) a = *reinterpret_cast<const u32x4*>(p);
+      else if (c + 8 <= C) a = __builtin_bit_cast(u32x4, ea_ld8u(p));
+      else {
+        f16x8 h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = c + j < C ? p[j] : (f16)0.0f;
+        a = __builtin_bit_cast(u32x4, h);
+      }
     } else if constexpr (XK == XK_F32) {
-      a = *reinterpret_cast<const u32x4*>((const float*)x + row * pitch + c);
-      b = *reinterpret_cast<const u32x4*>((const float*)x + row * pitch + c + 4);
+      const float* p = (const float*)x + row * pitch + c;
+      if (!ANY) {
+        a = *reinterpret_cast<const u32x4*>(p);
+        b = *reinterpret_cast<const u32x4*>(p + 4);
+      } else if (c + 8 <= C) {
+        a = __builtin_bit_cast(u32x4, ea_ld4u(p));
+        b = __builtin_bit_cast(u32x4, ea_ld4u(p + 4));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned u = c + j < C ? ea_f2u(p[j]) : 0u;
+          if (j < 4) a[j & 3] = u; else b[j & 3] = u;
+        }
+      }
     } else {
       const u32x2 w = *reinterpret_cast<const u32x2*>((const uint8_t*)x + row * pitch + c);
       a[0] = w[0];
@@ -200,47 +79,151 @@ struct Raw {
     }
   }
 };
-template <int XK>
-struct Raw<XK, 1> {
-  float a;
-  __device__ __forceinline__ void load(const void* x, const uint8_t* scale, long long row, int pitch, long long spitch, int c) {
-    ld_row<XK, 1>(x, scale, row, pitch, spitch, c, &a);
+template <bool ANY>
+__device__ __forceinline__ void ld_f32(const float* x, int c, int C, float* v) {
+  Row8<XK_F32, ANY> r;
+  r.load(x, nullptr, 0, 0, 0, c, C);
+  r.get(v);
+}
+template <bool F32, bool ANY>
+__device__ __forceinline__ void st_row8(void* x, long long at, int c, int C, const float* v) {
+  if constexpr (F32) {
+    float* d = (float*)x + at + c;
+    const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+    if (!ANY) {
+      *reinterpret_cast<f32x4*>(d) = lo;
+      *reinterpret_cast<f32x4*>(d + 4) = hi;
+      return;
+    }
+    if (c + 8 <= C) {
+      ea_st4u(d, lo);
+      ea_st4u(d + 4, hi);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < C) d[j] = v[j];
+  } else {
+    f16* d = (f16*)x + at + c;
+    f16x8 h;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = (f16)v[j];
+    if (!ANY) ea_st8(d, h);
+    else if (c + 8 <= C) ea_st8u(d, h);
+    else
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < C) d[j] = h[j];
   }
-  __device__ __forceinline__ void get(float* v) const { v[0] = a; }
+}
+
+// ------------------------------------------------------------------------------------------------------------ forward
+struct LnTrainParams {
+  const void* x; const float* gamma; const float* beta;
+  f16* y;                              // fp16 output
+  uint8_t* q; uint8_t* scale;          // 8-bit output
+  float* stats;                        // [M][2]: mean, 1 / sigma
+  int M, C, Kp; long long Rp;
+  float eps;
+};
+
+template <int XK, bool ANY, int LPR, int NV, bool OUT8>
+__global__ __launch_bounds__(256) void ea_ln_train_kernel(LnTrainParams p) {
+  constexpr int RPW = 64 / LPR;
+  const int lane = threadIdx.x & 63, sub = lane / LPR, l = lane % LPR;
+  const long long row = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW + sub;
+  const long long r = row < p.M ? row : p.M - 1;
+  float x[NV][8];
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * 8;
+    if (c < p.C) {
+      Row8<XK, ANY> w;
+      w.load(p.x, nullptr, r, p.C, 0, c, p.C);
+      w.get(x[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += x[i][j];
+  }
+  const float mean = ea_group_sum<LPR>(s) / (float)p.C;
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = (ANY ? c + j : c) < p.C ? x[i][j] - mean : 0.0f;
+      q += d * d;
+    }
+  }
+  const float rstd = 1.0f / sqrtf(ea_group_sum<LPR>(q) / (float)p.C + p.eps);
+  if (row < p.M && l == 0) *reinterpret_cast<f32x2*>(p.stats + 2 * row) = f32x2{mean, rstd};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * 8;
+    if (c < p.C) {
+      float ga[8], be[8];
+      ld_f32<ANY>(p.gamma, c, p.C, ga);
+      ld_f32<ANY>(p.beta, c, p.C, be);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i][j] = !ANY || c + j < p.C ? (x[i][j] - mean) * rstd * ga[j] + be[j] : 0.0f;
+      if (!OUT8 && row < p.M) st_row8<false, ANY>(p.y, row * p.C, c, p.C, x[i]);
+    }
+    if constexpr (OUT8) {                // a block of 128 columns: 16 lanes
+      int e;
+      const u32x2 w = ea_fp8_block<16>((const float*)x[i], e);
+      if (row < p.M && c < p.Kp) {
+        *reinterpret_cast<u32x2*>(p.q + row * p.Kp + c) = w;
+        if ((c & 127) == 0) p.scale[(long long)(c >> 7) * p.Rp + row] = (uint8_t)e;
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------- backward
+struct LnBwdParams {
+  const f16* dy; const void* x; const uint8_t* x_scale; const float* stats; const float* gamma;
+  const void* residual; void* dx;
+  float* part;                         // [gridDim.x][2][C]
+  int M, C, xpitch; long long xspitch;
 };
 
 // F32: the type of residual and dx
-template <int XK, bool F32, int VEC, int LPR, int NV>
-__global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
+template <int XK, bool F32, bool ANY, int LPR, int NV>
+__global__ __launch_bounds__(256, NV <= 3 ? 2 : 1) void ea_ln_bwd_kernel(LnBwdParams p) {
   constexpr int RPW = 64 / LPR;
   constexpr int RK = F32 ? XK_F32 : XK_F16;
-  constexpr bool KEEP = NV * VEC <= 24;      // a lane's share of a row stays in registers; a larger one is loaded twice, the second time from L2
+  constexpr bool KEEP = NV <= 3;       // a lane's share of a row stays in registers; a larger one is loaded twice, the second time from L2
   EA_SMEM(smem);
   float* red = reinterpret_cast<float*>(smem);      // [4][C]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, l = lane % LPR;
-  float ga[NV][VEC], ag[NV][VEC], ab[NV][VEC];
+  float ga[NV][8], ag[NV][8], ab[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (l + LPR * i) * VEC;
+    const int c = (l + LPR * i) * 8;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) ga[i][j] = ag[i][j] = ab[i][j] = 0.0f;
-    if (c < p.C) ld_f32<VEC>(p.gamma + c, ga[i]);
+    for (int j = 0; j < 8; ++j) ga[i][j] = ag[i][j] = ab[i][j] = 0.0f;
+    if (c < p.C) ld_f32<ANY>(p.gamma, c, p.C, ga[i]);
   }
   const float inv_c = 1.0f / (float)p.C;
   const long long stride = (long long)gridDim.x * 4 * RPW;
   constexpr int NR = KEEP ? NV : 1;
-  Raw<XK, VEC> rx[NR];
-  Raw<XK_F16, VEC> ry[NR];
-  Raw<RK, VEC> rr[NR];
+  Row8<XK, ANY> rx[NR];
+  Row8<XK_F16, ANY> ry[NR];
+  Row8<RK, ANY> rr[NR];
   f32x2 st;
   auto fetch1 = [&](long long row, int i, int k) {           // clamped, unconditional: the whole row's loads are in flight together
-    const int c0 = (l + LPR * i) * VEC, c = c0 < p.C ? c0 : 0;
-    rx[k].load(p.x, p.x_scale, row, p.xpitch, p.xspitch, c);
-    ry[k].load(p.dy, nullptr, row, p.C, 0, c);
+    const int c0 = (l + LPR * i) * 8, c = c0 < p.C ? c0 : 0;
+    rx[k].load(p.x, p.x_scale, row, p.xpitch, p.xspitch, c, p.C);
+    ry[k].load(p.dy, nullptr, row, p.C, 0, c, p.C);
   };
   auto fetch_res = [&](long long row, int i, int k) {
-    const int c0 = (l + LPR * i) * VEC, c = c0 < p.C ? c0 : 0;
-    rr[k].load(p.residual, nullptr, row, p.C, 0, c);
+    const int c0 = (l + LPR * i) * 8, c = c0 < p.C ? c0 : 0;
+    rr[k].load(p.residual, nullptr, row, p.C, 0, c, p.C);
   };
   auto fetch = [&](long long base) {
     const long long r = base + sub < p.M ? base + sub : p.M - 1;
@@ -256,21 +239,21 @@ __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
     const bool live = row < p.M;
     const long long r = live ? row : p.M - 1;
     const float mean = st[0], rs = st[1];
-    float n[NR][VEC], g[NR][VEC];
+    float n[NR][8], g[NR][8];
     float s1 = 0.0f, s2 = 0.0f;
     if (KEEP && p.residual)
 #pragma unroll
       for (int i = 0; i < NV; ++i) fetch_res(r, i, KEEP ? i : 0);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (l + LPR * i) * VEC, k = KEEP ? i : 0;
+      const int c = (l + LPR * i) * 8, k = KEEP ? i : 0;
       if (!KEEP) fetch1(r, i, 0);
       rx[k].get(n[k]);
       ry[k].get(g[k]);
-      const bool there = live && c < p.C;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = there ? g[k][j] : 0.0f;              // (a row or column that is not there adds nothing, whatever was read)
+      for (int j = 0; j < 8; ++j) {
+        const bool there = live && (ANY ? c + j : c) < p.C;  // (a row or column that is not there adds nothing, whatever was read)
+        const float d = there ? g[k][j] : 0.0f;
         n[k][j] = there ? (n[k][j] - mean) * rs : 0.0f;
         ag[i][j] += d * n[k][j];
         ab[i][j] += d;
@@ -285,7 +268,7 @@ __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
     if (live) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (l + LPR * i) * VEC, k = KEEP ? i : 0;
+        const int c = (l + LPR * i) * 8, k = KEEP ? i : 0;
         if (c >= p.C) continue;
         if (!KEEP) {
           fetch1(r, i, 0);
@@ -293,32 +276,18 @@ __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
           ry[0].get(g[0]);
           if (p.residual) fetch_res(r, i, 0);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
+          for (int j = 0; j < 8; ++j) {
             n[0][j] = (n[0][j] - mean) * rs;
             g[0][j] *= ga[i][j];
           }
         }
-        float o[VEC], res[VEC];
+        float o[8], res[8];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) res[j] = 0.0f;
+        for (int j = 0; j < 8; ++j) res[j] = 0.0f;
         if (p.residual) rr[k].get(res);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = rs * (g[k][j] - s1 - n[k][j] * s2) + res[j];
-        if constexpr (F32) {
-          float* d = (float*)p.dx + row * p.C + c;
-          if constexpr (VEC == 8) {
-            *reinterpret_cast<f32x4*>(d) = f32x4{o[0], o[1], o[2], o[3]};
-            *reinterpret_cast<f32x4*>(d + 4) = f32x4{o[4], o[5], o[6], o[7]};
-          } else *d = o[0];
-        } else {
-          f16* d = (f16*)p.dx + row * p.C + c;
-          if constexpr (VEC == 8) {
-            f16x8 h;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = (f16)o[j];
-            ea_st8(d, h);
-          } else *d = (f16)o[0];
-        }
+        for (int j = 0; j < 8; ++j) o[j] = rs * (g[k][j] - s1 - n[k][j] * s2) + res[j];
+        st_row8<F32, ANY>(p.dx, row * p.C, c, p.C, o);
       }
     }
   }
@@ -328,13 +297,13 @@ __global__ __launch_bounds__(256) void ea_ln_bwd_kernel(LnBwdParams p) {
     if (half) __syncthreads();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (l + LPR * i) * VEC;
+      const int c = (l + LPR * i) * 8;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
+      for (int j = 0; j < 8; ++j) {
         float v = half ? ab[i][j] : ag[i][j];
 #pragma unroll
         for (int m = LPR; m < 64; m <<= 1) v += ea_shfl_xor(v, m);
-        if (sub == 0 && c < p.C) red[wave * p.C + c + j] = v;
+        if (sub == 0 && c + j < p.C) red[wave * p.C + c + j] = v;
       }
     }
     __syncthreads();
@@ -365,51 +334,45 @@ __global__ __launch_bounds__(1024) void ea_ln_join_kernel(const float* part, flo
 bool ln_vec(int C, const void* a, const void* b, const void* c, const void* d, const void* e, const void* f) {
   return (C & 7) == 0 && ((((uintptr_t)a) | ((uintptr_t)b) | ((uintptr_t)c) | ((uintptr_t)d) | ((uintptr_t)e) | ((uintptr_t)f)) & 15) == 0;
 }
-// lanes per row; scalars always take the wave
-int ln_lanes(int C, bool vec) { return !vec ? 64 : C <= 384 ? 16 : C <= 768 ? 32 : 64; }
+int ln_lanes(int C) { return C <= 384 ? 16 : C <= 768 ? 32 : 64; }       // lanes per row
 
-template <int XK, bool OUT8>
-int ln_train_launch(const LnTrainParams& p, bool vec, void* stream) {
-  void (*k)(LnTrainParams);
-  const int lpr = ln_lanes(p.C, vec);
-  if (vec) {
-    k = lpr == 16 ? ea_ln_train_kernel<XK, 8, 16, 3, OUT8> : lpr == 32 ? ea_ln_train_kernel<XK, 8, 32, 3, OUT8>
-      : p.C <= 1536 ? ea_ln_train_kernel<XK, 8, 64, 3, OUT8> : p.C <= 2560 ? ea_ln_train_kernel<XK, 8, 64, 5, OUT8>
-      : ea_ln_train_kernel<XK, 8, 64, 8, OUT8>;
-  } else {
-    k = p.C <= 512 ? ea_ln_train_kernel<XK, 1, 64, 8, OUT8> : p.C <= 1536 ? ea_ln_train_kernel<XK, 1, 64, 24, OUT8>
-      : ea_ln_train_kernel<XK, 1, 64, 64, OUT8>;
-  }
-  const int rows = 4 * (64 / lpr);
+template <int XK, bool ANY, bool OUT8>
+int ln_train_launch(const LnTrainParams& p, void* stream) {
+  const int lpr = ln_lanes(p.C), rows = 4 * (64 / lpr);
+  auto k = lpr == 16 ? ea_ln_train_kernel<XK, ANY, 16, 3, OUT8> : lpr == 32 ? ea_ln_train_kernel<XK, ANY, 32, 3, OUT8>
+         : p.C <= 1536 ? ea_ln_train_kernel<XK, ANY, 64, 3, OUT8> : p.C <= 2560 ? ea_ln_train_kernel<XK, ANY, 64, 5, OUT8>
+         : ea_ln_train_kernel<XK, ANY, 64, 8, OUT8>;
   EA_LAUNCH(k, dim3((p.M + rows - 1) / rows), dim3(256), 0, stream, p);
   return ea_launch_status();
+}
+template <int XK>
+int ln_train_pick(const LnTrainParams& p, bool vec, void* stream) {
+  if (vec) return p.q ? ln_train_launch<XK, false, true>(p, stream) : ln_train_launch<XK, false, false>(p, stream);
+  return p.q ? ln_train_launch<XK, true, true>(p, stream) : ln_train_launch<XK, true, false>(p, stream);
 }
 
 // Workgroups of the backward pass: as many as are resident (two per CU up to 1536 columns, one above), each walking the rows.  us for
 // 256 / 512 / 1024: 32768 x 320 23.1 / 22.8 / 28.3, 32768 x 1280 47.8 / 45.1 / 49.2, 4096 x 4096 34.9 / 43.1 / 60.9.
-int ln_bwd_grid(int M, int C) {            // the same for both paths of a width: the workspace does not depend on alignment
-  const int rows = 4 * (64 / ln_lanes(C, (C & 7) == 0));
+int ln_bwd_grid(int M, int C) {
+  const int rows = 4 * (64 / ln_lanes(C));
   const int g = (M + rows - 1) / rows;
   const int most = C > 1536 ? 256 : 512;
   return g < most ? g : most;
 }
 
-template <int XK, bool F32>
-int ln_bwd_launch(const LnBwdParams& p, bool vec, int grid, void* stream) {
-  void (*k)(LnBwdParams);
-  const int lpr = ln_lanes(p.C, vec);
-  if (vec) {
-    k = lpr == 16 ? ea_ln_bwd_kernel<XK, F32, 8, 16, 3> : lpr == 32 ? ea_ln_bwd_kernel<XK, F32, 8, 32, 3>
-      : p.C <= 1536 ? ea_ln_bwd_kernel<XK, F32, 8, 64, 3> : p.C <= 2560 ? ea_ln_bwd_kernel<XK, F32, 8, 64, 5>
-      : ea_ln_bwd_kernel<XK, F32, 8, 64, 8>;
-  } else {
-    k = p.C <= 512 ? ea_ln_bwd_kernel<XK, F32, 1, 64, 8> : p.C <= 1536 ? ea_ln_bwd_kernel<XK, F32, 1, 64, 24>
-      : ea_ln_bwd_kernel<XK, F32, 1, 64, 64>;
-  }
-  const int smem = 4 * p.C * (int)sizeof(float);
+template <int XK, bool F32, bool ANY>
+int ln_bwd_launch(const LnBwdParams& p, int grid, void* stream) {
+  const int lpr = ln_lanes(p.C), smem = 4 * p.C * (int)sizeof(float);
+  auto k = lpr == 16 ? ea_ln_bwd_kernel<XK, F32, ANY, 16, 3> : lpr == 32 ? ea_ln_bwd_kernel<XK, F32, ANY, 32, 3>
+         : p.C <= 1536 ? ea_ln_bwd_kernel<XK, F32, ANY, 64, 3> : p.C <= 2560 ? ea_ln_bwd_kernel<XK, F32, ANY, 64, 5>
+         : ea_ln_bwd_kernel<XK, F32, ANY, 64, 8>;
   ea_allow_big_lds(k, smem);
   EA_LAUNCH(k, dim3(grid), dim3(256), smem, stream, p);
   return ea_launch_status();
+}
+template <int XK, bool F32>
+int ln_bwd_pick(const LnBwdParams& p, bool vec, int grid, void* stream) {
+  return vec ? ln_bwd_launch<XK, F32, false>(p, grid, stream) : ln_bwd_launch<XK, F32, true>(p, grid, stream);
 }
 
 }  // namespace
@@ -423,8 +386,7 @@ extern "C" int ea_layernorm_train(const void* x, int in_f32, const float* gamma,
   p.x = x; p.gamma = gamma; p.beta = beta; p.y = (f16*)y; p.q = (uint8_t*)q; p.scale = scale; p.stats = stats;
   p.M = M; p.C = C; p.Kp = ea_fp8_blocks(C) * EA_FP8_BLOCK; p.Rp = ea_fp8_scale_pitch(M); p.eps = eps;
   const bool vec = ln_vec(C, x, gamma, beta, y, nullptr, nullptr);
-  if (in_f32) return q ? ln_train_launch<XK_F32, true>(p, vec, stream) : ln_train_launch<XK_F32, false>(p, vec, stream);
-  return q ? ln_train_launch<XK_F16, true>(p, vec, stream) : ln_train_launch<XK_F16, false>(p, vec, stream);
+  return in_f32 ? ln_train_pick<XK_F32>(p, vec, stream) : ln_train_pick<XK_F16>(p, vec, stream);
 }
 
 extern "C" size_t ea_layernorm_bwd_workspace_bytes(int M, int C) {
@@ -447,8 +409,8 @@ extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const
   p.xspitch = ea_fp8_scale_pitch(M);
   const bool vec = ln_vec(C, dy, x, gamma, residual, dx, nullptr);
   const int grid = ln_bwd_grid(M, C);
-  const int st = x_kind == XK_F16 ? ln_bwd_launch<XK_F16, false>(p, vec, grid, stream)
-               : x_kind == XK_F32 ? ln_bwd_launch<XK_F32, true>(p, vec, grid, stream) : ln_bwd_launch<XK_FP8, false>(p, vec, grid, stream);
+  const int st = x_kind == XK_F16 ? ln_bwd_pick<XK_F16, false>(p, vec, grid, stream)
+               : x_kind == XK_F32 ? ln_bwd_pick<XK_F32, true>(p, vec, grid, stream) : ln_bwd_pick<XK_FP8, false>(p, vec, grid, stream);
   if (st != EA_OK) return st;
   auto k = ea_ln_join_kernel;
   EA_LAUNCH(k, dim3((2 * C + 31) / 32), dim3(1024), 32 * 33 * sizeof(float), stream, (const float*)workspace, dgamma, dbeta, grid, C);

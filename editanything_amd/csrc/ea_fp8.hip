@@ -220,7 +220,7 @@ struct ActParams {
 };
 
 template <int ACT>
-__device__ __forceinline__ float act_f(float z) { return ACT == EA_ACT_SILU ? ea_silu(z) : ea_gelu_erf(z); }
+__device__ __forceinline__ float act_f(float z) { return ACT == EA_ACT_SILU ? ea_silu(z) : ea_fp8_gelu(z); }
 
 // Phi(x) and x phi(x); 1 - Phi(a) = erfc(a / sqrt 2) / 2 as in ea_gelu_erf
 __device__ __forceinline__ void gelu_parts(float x, float& phi_c, float& xp) {

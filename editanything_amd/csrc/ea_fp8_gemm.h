@@ -125,7 +125,7 @@ __device__ __forceinline__ void ea_fp8_start(const EaFp8GemmParams& p, f32x4 (&a
 
 template <int ACT>
 __device__ __forceinline__ float ea_fp8_act(float x) {
-  return ACT == EA_ACT_SILU ? ea_silu(x) : ACT == EA_ACT_GELU ? ea_gelu_erf(x) : x;
+  return ACT == EA_ACT_SILU ? ea_silu(x) : ACT == EA_ACT_GELU ? ea_fp8_gelu(x) : x;
 }
 // 16-byte accesses.  m0: the workgroup's first row, mw: the wave's
 template <int ACT, int FM, int FN, int FMG, int FNG>
@@ -164,7 +164,10 @@ __device__ __forceinline__ void ea_fp8_finish_vec(const EaFp8GemmParams& p, cons
       const unsigned o = oc[g] + row(i) * oline;
       float v[8];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) v[c] = ea_fp8_act<ACT>(acc[i][j + c / 4][c % 4]) * p.scale;
+      for (int c = 0; c < 8; ++c) v[c] = ea_fp8_act<ACT>(acc[i][j + c / 4][c % 4]);
+      if (p.scale != 1.0f)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] *= p.scale;
       if (p.residual) {
         const f16x8 r = __builtin_bit_cast(f16x8, r0[i & 1][g]);
 #pragma unroll
@@ -206,7 +209,7 @@ __device__ __forceinline__ void ea_fp8_finish(const EaFp8GemmParams& p, const f3
         const int m = mw + 16 * FMG * (i / FMG) + FMG * l15 + i % FMG, n = n0 + 16 * FNG * (j / FNG) + 4 * FNG * lq + 4 * (j % FNG) + r;
         float v = acc[i][j][r];
         if (m >= p.M || n >= p.N) continue;
-        v = (p.act == EA_ACT_GELU ? ea_gelu_erf(v) : p.act == EA_ACT_SILU ? ea_silu(v) : v) * p.scale;
+        v = (p.act == EA_ACT_GELU ? ea_fp8_gelu(v) : p.act == EA_ACT_SILU ? ea_silu(v) : v) * p.scale;
         if (p.residual) v += (float)p.residual[(long long)m * p.ldr + n];
         else if (p.residual32) v += p.residual32[(long long)m * p.ldr + n];
         if (p.out_f32) ((float*)p.out)[(long long)m * p.ldc + n] = v;

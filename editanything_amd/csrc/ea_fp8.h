@@ -228,5 +228,6 @@ __device__ __forceinline__ float ea_fp8_gelu(float x) {
   return (x < 0.0f ? 0.0f : x) - a * ea_exp2_raw(-a * q - 1.0f);
 }
 
+#define EA_FP8_ROWS (1 << 30)      // most rows of an entry that counts them in 32 bits: tile counts and row indexes stay below 2^31
 static inline int ea_fp8_blocks(int cols) { return (cols + EA_FP8_BLOCK - 1) / EA_FP8_BLOCK; }
 static inline long long ea_fp8_scale_pitch(long long rows) { return (rows + 15) / 16 * 16; }

@@ -279,13 +279,15 @@ __device__ __forceinline__ f16 wl_factor(int byte) {
   return __builtin_bit_cast(f16, u);
 }
 
-// an MFMA operand whose row q is ones: row q of the product is then the column sums of the other operand
-__device__ __forceinline__ f16x8 wl_unit_row(int q, int l15) {
-  unsigned u = l15 == q ? 0x3c003c00u : 0u;
-#ifndef EA_EMU
-  asm volatile("" : "+v"(u));              // (made where it is used: kept over the loop, its four registers were spilled)
-#endif
-  return __builtin_bit_cast(f16x8, u32x4{u, u, u, u});
+// A lane's share of db: the 8 rows that a dy fragment holds of its column.  On the vector unit, beside the products: summed by the matrix
+// unit with a row of ones, two fragments in one accumulator, the zeros of one's operand times an infinity of the other's column made NaN.
+__device__ __forceinline__ void wl_sum8(float& s, f16x8 v) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s += (float)v[j];
+}
+__device__ __forceinline__ float wl_sum_rows(float s) {     // lanes l15, + 16, + 32, + 48 hold the other rows of the column
+  s += ea_shfl_xor(s, 16);
+  return s + ea_shfl_xor(s, 32);
 }
 
 // ------------------------------------------------------------------------------------- weight gradient, 128 x 128 tiles
@@ -328,7 +330,8 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
     ad[i] = r * 256 + (((wm * 4 + (i ^ (2 * wn))) ^ wl_dy_swz(r)) << 5) + (l15 & 3) * 8;
     ax[i] = WR_DY + s * 128 + (((wn * 4 + i) ^ wl_x_swz(s)) << 4) + (l15 & 1) * 8;
   }
-  f32x4 acc[4][4], accb = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 acc[4][4];
+  float colsum[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -377,8 +380,8 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][j] = ea_mfma_16x16x32(fx[j][ks], fa[i][ks], acc[i][j]);
         if (sums) {
-          accb = ea_mfma_16x16x32(wl_unit_row(0, l15), fa[0][ks], accb);
-          accb = ea_mfma_16x16x32(wl_unit_row(1, l15), fa[1][ks], accb);
+          wl_sum8(colsum[0], fa[0][ks]);
+          wl_sum8(colsum[1], fa[1][ks]);
         }
       }
     }
@@ -388,10 +391,13 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
 #pragma unroll
   for (int i = 0; i < 4; ++i) {            // D^T: a lane holds 4 consecutive k of one n
     const int n = n0 + wm * 64 + (i ^ (2 * wn)) * 16 + l15;
+    if (i < 2 && sums) {
+      const float t = wl_sum_rows(colsum[i & 1]);
+      if (n < p.N && lq == 0) db[n] = t;
+    }
     if (n >= p.N) continue;
 #pragma unroll
     for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wn * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
-    if (i < 2 && sums && lq == 0) db[n] = accb[i];
   }
 }
 
@@ -447,7 +453,8 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
   };
   auto stage_x = [&](int h) { wl_dma16(rx, vx[h] + ox, sbuf + WL_DY + h * 8192 + wave * 1024); };
 
-  f32x4 acc[8][4], accb = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 acc[8][4];
+  float colsum[2] = {0.0f, 0.0f};       // of quadrants 0 and 1
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -495,9 +502,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[qa * 4 + i][qb * 2 + j] = ea_mfma_16x16x32(fb[j][ks], fa[i][ks], acc[qa * 4 + i][qb * 2 + j]);
-      if (sums) {                          // row qa of the other operand is ones: D's row qa is the column sums of quadrant qa
-        accb = ea_mfma_16x16x32(wl_unit_row(qa, l15), fa[0][ks], accb);
-      }
+      if (sums) wl_sum8(colsum[qa], fa[0][ks]);
     }
 #ifndef EA_EMU
     __builtin_amdgcn_s_setprio(0);
@@ -575,11 +580,12 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
 #pragma unroll
     for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wn * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
   }
-  if (sums && lq == 0)
+  if (sums)
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int n = n0 + wm * 128 + q * 64 + wn * 16 + l15;
-      if (n < p.N) db[n] = accb[q];
+      const float t = wl_sum_rows(colsum[q]);
+      if (n < p.N && lq == 0) db[n] = t;
     }
 }
 
@@ -675,7 +681,7 @@ int fp8_launch(EaFp8GemmParams& p, void* stream) {
 extern "C" int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K,
                            const ea_epilogue* e, void* stream) {
   if (!a || !a_scale || !w || !w_scale || !e || !e->out) return EA_ERR_BAD_ARG;
-  if (M <= 0 || N <= 0 || K <= 0 || K > (1 << 20)) return EA_ERR_BAD_SHAPE;
+  if (M <= 0 || N <= 0 || K <= 0 || M > EA_FP8_ROWS || N > (1 << 22) || K > (1 << 20)) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)a & 15) || ((uintptr_t)w & 15) || ((uintptr_t)a_scale & 3)) return EA_ERR_BAD_ARG;
   if (e->act != EA_ACT_NONE && e->act != EA_ACT_SILU && e->act != EA_ACT_GELU) return EA_ERR_UNSUPPORTED;
   if (e->bias_per_row || e->rowvec || e->row_scale || e->ln_stats || e->row_stats_out || e->gn_stats_out || e->gn_next_out || e->acc_scale_k)
@@ -695,7 +701,7 @@ extern "C" int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const vo
 }
 
 extern "C" size_t ea_gemm_fp8_wgrad_workspace_bytes(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || M > EA_FP8_ROWS) return 0;
   const int s = wgrad_plan(M, N, K).splits;
   return s == 1 ? 0 : (size_t)s * ((((size_t)N * K + N) + 3) & ~(size_t)3) * sizeof(float);
 }
@@ -703,7 +709,7 @@ extern "C" size_t ea_gemm_fp8_wgrad_workspace_bytes(int M, int N, int K) {
 extern "C" int ea_gemm_fp8_wgrad(const void* dy, const void* x, const unsigned char* x_scale, float* dw, float* db, int M, int N, int K,
                                  void* workspace, size_t ws_bytes, void* stream) {
   if (!dy || !x || !x_scale || !dw || !db) return EA_ERR_BAD_ARG;
-  if (M <= 0 || N <= 0 || K <= 0 || N > (1 << 20) || K > (1 << 20)) return EA_ERR_BAD_SHAPE;
+  if (M <= 0 || N <= 0 || K <= 0 || M > EA_FP8_ROWS || N > (1 << 20) || K > (1 << 20)) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)x & 15) || ((uintptr_t)dw & 15) || ((uintptr_t)workspace & 15)) return EA_ERR_BAD_ARG;
   if (ws_bytes < ea_gemm_fp8_wgrad_workspace_bytes(M, N, K) || (!workspace && ws_bytes)) return EA_ERR_WORKSPACE;
   WgradParams p;

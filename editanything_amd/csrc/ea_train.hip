@@ -380,7 +380,7 @@ int ln_bwd_pick(const LnBwdParams& p, bool vec, int grid, void* stream) {
 extern "C" int ea_layernorm_train(const void* x, int in_f32, const float* gamma, const float* beta, float eps, void* y, void* q,
                                   unsigned char* scale, float* stats, int M, int C, void* stream) {
   if (!x || !gamma || !beta || !stats || (!y == !q) || (q && !scale)) return EA_ERR_BAD_ARG;
-  if (M <= 0 || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
+  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)stats & 7) || ((uintptr_t)q & 15)) return EA_ERR_BAD_ARG;
   LnTrainParams p;
   p.x = x; p.gamma = gamma; p.beta = beta; p.y = (f16*)y; p.q = (uint8_t*)q; p.scale = scale; p.stats = stats;
@@ -390,7 +390,7 @@ extern "C" int ea_layernorm_train(const void* x, int in_f32, const float* gamma,
 }
 
 extern "C" size_t ea_layernorm_bwd_workspace_bytes(int M, int C) {
-  if (M <= 0 || C <= 0 || C > 4096) return 0;
+  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096) return 0;
   return (size_t)ln_bwd_grid(M, C) * 2 * C * sizeof(float);
 }
 
@@ -399,7 +399,7 @@ extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const
                                 void* workspace, size_t ws_bytes, void* stream) {
   if (!dy || !x || !stats || !gamma || !dx || !dgamma || !dbeta || !workspace || (x_kind == XK_FP8 && !x_scale)) return EA_ERR_BAD_ARG;
   if (x_kind < XK_F16 || x_kind > XK_FP8) return EA_ERR_BAD_ARG;
-  if (M <= 0 || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
+  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)stats & 7) || ((uintptr_t)workspace & 3)) return EA_ERR_BAD_ARG;
   if (ws_bytes < ea_layernorm_bwd_workspace_bytes(M, C)) return EA_ERR_WORKSPACE;
   LnBwdParams p;

@@ -1031,6 +1031,9 @@ _F16, _F32, _U8, _E4M3 = torch.float16, torch.float32, torch.uint8, torch.float8
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
 
 
+_MOST_ROWS = 1 << 30           # of an entry that counts rows in 32 bits
+
+
 def _refuse(rule, **given):
     """ValueError with the rule that was broken and what was given."""
     def show(v):
@@ -1165,8 +1168,8 @@ def layernorm_train(x, gamma, beta, eps=1e-5, fp8=False):
     x fp16 / fp32 [..., C]; gamma, beta fp32 [C].  -> (y, stats): y fp16, or with `fp8` an Fp8Tensor (the next product's operand and its
     weight gradient's input, written in the same pass); stats fp32 [rows, 2] = (mean, 1 / sigma)."""
     M, Cc = _lead(x, (_F16, _F32))
-    if not (0 < Cc <= 4096 and gamma.dtype == beta.dtype == _F32 and gamma.shape == beta.shape == (Cc,)):
-        _refuse("layernorm_train: x must be fp16 or fp32 [..., C <= 4096], gamma and beta fp32 [C]", x=x, gamma=gamma, beta=beta)
+    if not (0 < Cc <= 4096 and M <= _MOST_ROWS and gamma.dtype == beta.dtype == _F32 and gamma.shape == beta.shape == (Cc,)):
+        _refuse("layernorm_train: x must be fp16 or fp32 [..., C <= 4096] of at most 2^30 rows, gamma and beta fp32 [C]", x=x, gamma=gamma, beta=beta)
     dev = x.device
     _on_device(dev, x, gamma, beta)
     stats = torch.empty_strided((M, 2), (2, 1), dtype=_F32, device=dev)
@@ -1186,9 +1189,9 @@ def layernorm_backward(dy, x, stats, gamma, residual=None):
     q8 = _is_rows(x)
     kind = 2 if q8 else 0 if not torch.is_tensor(x) else 1 if x.dtype == _F32 else 0
     out = _F32 if kind == 1 else _F16
-    if not (0 < Cc <= 4096 and (q8 or (torch.is_tensor(x) and x.dtype == out)) and x.shape == dy.shape and gamma.dtype == stats.dtype == _F32
+    if not (0 < Cc <= 4096 and M <= _MOST_ROWS and (q8 or (torch.is_tensor(x) and x.dtype == out)) and x.shape == dy.shape and gamma.dtype == stats.dtype == _F32
             and gamma.shape == (Cc,) and stats.shape == (M, 2) and (residual is None or (residual.dtype == out and residual.shape == dy.shape))):
-        _refuse("layernorm_backward: dy must be fp16 [..., C <= 4096], x fp16, fp32 or an Fp8Tensor of rows of dy's shape, stats fp32 [rows, 2], "
+        _refuse("layernorm_backward: dy must be fp16 [..., C <= 4096] of at most 2^30 rows, x fp16, fp32 or an Fp8Tensor of rows of dy's shape, stats fp32 [rows, 2], "
                 "gamma fp32 [C], residual of dy's shape and of x's type (fp16 for an Fp8Tensor)", dy=dy, x=x, stats=stats, gamma=gamma,
                 residual=residual)
     dev = dy.device
@@ -1246,9 +1249,10 @@ def gemm_fp8(a, w, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=t
     """out = residual + scale * act(a w^T + bias): a an Fp8Tensor of rows [..., K], w an Fp8Tensor weight [N, K]; bias fp32 [N]; act
     ACT_NONE, ACT_SILU or ACT_GELU; residual fp16 or fp32 [..., N] (may be `out`); out fp16 or fp32.  The accumulators are fp32; the matrix
     unit adds eight neighbouring products at a time, each kept to 2^-13 of the largest of the eight."""
-    if not (_is_rows(a) and isinstance(w, Fp8Tensor) and w.block_rows == 128 and a.cols == w.cols and act in (ACT_NONE, ACT_SILU, ACT_GELU)):
-        _refuse("gemm_fp8: a must be an Fp8Tensor of rows [..., K] (quantize_fp8), w an Fp8Tensor weight [N, K] (quantize_fp8_weight), act ACT_NONE, "
-                "ACT_SILU or ACT_GELU", a=a, w=w, act=act)
+    if not (_is_rows(a) and a.rows <= _MOST_ROWS and isinstance(w, Fp8Tensor) and w.block_rows == 128 and a.cols == w.cols
+            and act in (ACT_NONE, ACT_SILU, ACT_GELU)):
+        _refuse("gemm_fp8: a must be an Fp8Tensor of at most 2^30 rows [..., K] (quantize_fp8), w an Fp8Tensor weight [N, K] (quantize_fp8_weight), act "
+                "ACT_NONE, ACT_SILU or ACT_GELU", a=a, w=w, act=act)
     M, N, dev = a.rows, w.rows, a.q.device
     shape = a.shape[:-1] + (N,)
     if not (out_dtype in (_F16, _F32) and (bias is None or (bias.dtype == _F32 and bias.shape == (N,)))
@@ -1276,8 +1280,8 @@ def gemm_fp8_wgrad(dy, x):
     """Gradients of a Linear's weight and bias from its 8-bit input: dy fp16 [..., N], x an Fp8Tensor of rows [..., K] (|values| <=
     114688) -> (dw fp32 [N, K] = dy^T x, db fp32 [N]), both summed in fp32 in a fixed order."""
     M, N = _lead(dy, (_F16,))
-    if not (N and _is_rows(x) and x.rows == M):
-        _refuse("gemm_fp8_wgrad: dy must be fp16 [..., N], x an Fp8Tensor of as many rows", dy=dy, x=x)
+    if not (N and M <= _MOST_ROWS and _is_rows(x) and x.rows == M):
+        _refuse("gemm_fp8_wgrad: dy must be fp16 [..., N] of at most 2^30 rows, x an Fp8Tensor of as many rows", dy=dy, x=x)
     K, dev = x.cols, dy.device
     _on_device(dev, dy, x.q, x.scale)
     if not M:

@@ -530,7 +530,51 @@ def test_gemm_fp8_wgrad_range(kb):
     assert np.abs(kb.down(dw)[:4] - values(q, e, 128)).max() <= 2.0 ** -24 and kb.down(dw)[0, 0] == 65536
 
 
+@pytest.mark.parametrize("kernel", [0, 101, 102, 103])
+def test_gemm_fp8_wgrad_keeps_nan_and_infinity_in_their_row_and_column(kb, kernel):
+    """An infinity in dy column n and a NaN code in x column k: row n and column k of dw and db[n] alone show them."""
+    M, N, K = 70, 264, 300
+    force(kb, kernel)
+    q, e = quantize(rows(19, M, K, np.float32))
+    dy = rows(20, M, N, np.float16, 0.05)
+    q[9, 140] = 0x7f
+    cols = [21, 77, 200]
+    dy[[3, 40, 69], cols] = np.inf, np.nan, -np.inf
+    dw, db = kb.zeros((N, K), np.float32), kb.zeros((N,), np.float32)
+    nbytes = kb.lib.ea_gemm_fp8_wgrad_workspace_bytes(M, N, K)
+    ws = kb.zeros((nbytes // 4,), np.float32) if nbytes else None
+    assert kb.lib.ea_gemm_fp8_wgrad(ptr(dy), ptr(q), ptr(pack_scales(e)), ptr(dw), ptr(db), M, N, K, ptr(ws), nbytes, kb.stream) == 0
+    gw, gb = np.isfinite(kb.down(dw)), np.isfinite(kb.down(db))
+    want = np.ones((N, K), bool)
+    want[:, 140] = want[cols] = False
+    assert np.array_equal(gw, want) and np.array_equal(gb, want[:, 0])
+
+
 # ------------------------------------------------------------------------------------------------------------------ refusals
+def test_more_rows_than_an_index_holds_are_refused(emu_lib):
+    """Rows counted in 32 bits end at 2^30; nothing is read before the refusal."""
+    a = np.zeros((256, 256), np.float32)
+    p, big = a.ctypes.data, (1 << 30) + 1
+    e = epilogue(a)
+    assert emu_lib.ea_layernorm_train(p, 0, p, p, 1e-5, p, None, None, p, big, 8, None) == -1
+    assert emu_lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, p, p, p, big, 8, p, 1 << 40, None) == -1
+    assert emu_lib.ea_layernorm_bwd_workspace_bytes(big, 8) == 0
+    assert emu_lib.ea_gemm_fp8(p, p, p, p, big, 16, 128, ctypes.byref(e), None) == -1
+    assert emu_lib.ea_gemm_fp8(p, p, p, p, 16, (1 << 22) + 1, 128, ctypes.byref(e), None) == -1
+    assert emu_lib.ea_gemm_fp8_wgrad(p, p, p, p, p, big, 16, 16, None, 0, None) == -1
+    assert emu_lib.ea_gemm_fp8_wgrad_workspace_bytes(big, 16, 16) == 0
+    one = torch.ones(8)
+    for n in (big, (1 << 32) + 5):             # (the second is 5 in 32 bits)
+        x = torch.zeros(1, 8, dtype=torch.float16).expand(n, 8)
+        t = ops.Fp8Tensor.__new__(ops.Fp8Tensor)
+        t.q, t.scale, t.cols, t.rows, t.shape, t.block_rows = torch.zeros(1, 128).to(torch.float8_e4m3fn), torch.zeros(1, 16), 8, n, (n, 8), 1
+        w = ops.Fp8Tensor(torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(1, 1, dtype=torch.uint8), 8)
+        for f in (lambda: ops.layernorm_train(x, one, one), lambda: ops.layernorm_backward(x, x, torch.zeros(1, 2).expand(n, 2), one),
+                  lambda: ops.gemm_fp8(t, w), lambda: ops.gemm_fp8_wgrad(x, t)):
+            with pytest.raises(ValueError, match="2\\^30"):
+                f()
+
+
 def test_the_c_entries_refuse(emu_lib):
     lib = emu_lib
     a = np.zeros((256, 256), np.float32)

@@ -13,11 +13,14 @@
 // (backward 32768 x 320: 55 us against 23).
 // The column sums stay in registers over all rows that a wave visits (a lane always owns the same columns), are joined over the
 // workgroup in LDS once, written as one partial per workgroup and joined by a second launch in a fixed order: no atomics, so a
-// run repeats bit for bit.  Measured (backward with residual): 16384 x 1280 fp32 52 us = 5.7 TB/s, 32768 x 1280 fp16 without residual
-// 45 us = 5.6 TB/s, 32768 x 320 fp16 23 us = 3.7 TB/s, 512 x 1280 9 us (two launches).  Forward: 32768 x 1280 fp16 30 us = 5.6 TB/s, into
-// 8 bits 28 us.  The next row is in flight while one is worked off (without: 16384 x 1280 64 us).
+// run repeats bit for bit.  Up to 1024 rows one launch does all of it (ea_ln_bwd_few_kernel).
+// Measured (backward with residual): 16384 x 1280 fp32 52 us = 5.7 TB/s, 32768 x 1280 fp16 without residual 45 us = 5.6 TB/s, 32768 x 320
+// fp16 23 us = 3.7 TB/s, 512 x 1280 3.7 us.  Forward: 32768 x 1280 fp16 30 us = 5.6 TB/s, into 8 bits 28 us.  The next row is in flight
+// while one is worked off (without: 16384 x 1280 64 us).
 #include "ea_fp8.h"
 #include "../../include/editanything_hip.h"
+
+int ea_forced_variant();          // ea_gemm.hip: the calling thread's ea_tuning.variant (tests)
 
 namespace {
 
@@ -331,6 +334,109 @@ __global__ __launch_bounds__(1024) void ea_ln_join_kernel(const float* part, flo
   if (gy == 0 && c < cols) (c < C ? dgamma[c] : dbeta[c - C]) = red[cx];
 }
 
+// Few rows: one launch.  The first workgroups take 32 columns each and walk all rows (64 row lanes x 4 lanes of 8 columns, four rows in
+// flight per lane) for dgamma and dbeta; the others take rows for dx.  Everything is read twice, the second time from a cache, and there is
+// no partial to join.
+constexpr int LF_COLS = 32, LF_U = 4, LF_LDS = 64 * 65 * 4;
+template <int XK, bool F32, bool ANY, int LPR, int NV>
+__global__ __launch_bounds__(256) void ea_ln_bwd_few_kernel(LnBwdParams p, float* dgamma, float* dbeta, int ncol) {
+  EA_SMEM(smem);
+  if ((int)blockIdx.x < ncol) {
+    float* red = reinterpret_cast<float*>(smem);      // [64 row lanes][dgamma | dbeta of 32 columns], padded by one
+    const int cl = threadIdx.x & 3, rl = threadIdx.x >> 2, c0 = blockIdx.x * LF_COLS, c = c0 + cl * 8, cc = c < p.C ? c : 0;
+    float ag[8], ab[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ag[j] = ab[j] = 0.0f;
+    for (int m0 = rl; m0 < p.M; m0 += 64 * LF_U) {
+      Row8<XK, ANY> rx[LF_U];
+      Row8<XK_F16, ANY> ry[LF_U];
+      f32x2 st[LF_U];
+#pragma unroll
+      for (int u = 0; u < LF_U; ++u) {
+        const int m = m0 + 64 * u < p.M ? m0 + 64 * u : p.M - 1;
+        rx[u].load(p.x, p.x_scale, m, p.xpitch, p.xspitch, cc, p.C);
+        ry[u].load(p.dy, nullptr, m, p.C, 0, cc, p.C);
+        st[u] = *reinterpret_cast<const f32x2*>(p.stats + 2ll * m);
+      }
+#pragma unroll
+      for (int u = 0; u < LF_U; ++u) {
+        float n[8], d[8];
+        rx[u].get(n);
+        ry[u].get(d);
+        if (m0 + 64 * u < p.M)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            ag[j] += d[j] * ((n[j] - st[u][0]) * st[u][1]);
+            ab[j] += d[j];
+          }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      red[rl * 65 + cl * 8 + j] = ag[j];
+      red[rl * 65 + 32 + cl * 8 + j] = ab[j];
+    }
+    __syncthreads();
+    const int k = threadIdx.x & 63, part = threadIdx.x >> 6;
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += red[(part * 16 + i) * 65 + k];
+    __syncthreads();
+    red[part * 65 + k] = t;
+    __syncthreads();
+    if (part == 0 && c0 + (k & 31) < p.C) (k < 32 ? dgamma : dbeta)[c0 + (k & 31)] = (red[k] + red[65 + k]) + (red[130 + k] + red[195 + k]);
+    return;
+  }
+  constexpr int RPW = 64 / LPR;
+  constexpr int RK = F32 ? XK_F32 : XK_F16;
+  const int lane = threadIdx.x & 63, sub = lane / LPR, l = lane % LPR;
+  const int row = (((int)blockIdx.x - ncol) * 4 + (threadIdx.x >> 6)) * RPW + sub, r = row < p.M ? row : p.M - 1;
+  Row8<XK, ANY> rx[NV];
+  Row8<XK_F16, ANY> ry[NV];
+  Row8<RK, ANY> rr[NV];
+  const f32x2 st = *reinterpret_cast<const f32x2*>(p.stats + 2ll * r);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c0 = (l + LPR * i) * 8, c = c0 < p.C ? c0 : 0;
+    rx[i].load(p.x, p.x_scale, r, p.xpitch, p.xspitch, c, p.C);
+    ry[i].load(p.dy, nullptr, r, p.C, 0, c, p.C);
+    if (p.residual) rr[i].load(p.residual, nullptr, r, p.C, 0, c, p.C);
+  }
+  float n[NV][8], g[NV][8], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * 8;
+    float ga[8];
+    ld_f32<ANY>(p.gamma, c < p.C ? c : 0, p.C, ga);
+    rx[i].get(n[i]);
+    ry[i].get(g[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool there = (ANY ? c + j : c) < p.C;
+      n[i][j] = there ? (n[i][j] - st[0]) * st[1] : 0.0f;
+      g[i][j] = there ? g[i][j] * ga[j] : 0.0f;
+      s1 += g[i][j];
+      s2 += g[i][j] * n[i][j];
+    }
+  }
+  const float inv_c = 1.0f / (float)p.C;
+  s1 = ea_group_sum<LPR>(s1) * inv_c;
+  s2 = ea_group_sum<LPR>(s2) * inv_c;
+  if (row >= p.M) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (l + LPR * i) * 8;
+    if (c >= p.C) continue;
+    float o[8], res[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) res[j] = 0.0f;
+    if (p.residual) rr[i].get(res);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = st[1] * (g[i][j] - s1 - n[i][j] * s2) + res[j];
+    st_row8<F32, ANY>(p.dx, (long long)row * p.C, c, p.C, o);
+  }
+}
+
 bool ln_vec(int C, const void* a, const void* b, const void* c, const void* d, const void* e, const void* f) {
   return (C & 7) == 0 && ((((uintptr_t)a) | ((uintptr_t)b) | ((uintptr_t)c) | ((uintptr_t)d) | ((uintptr_t)e) | ((uintptr_t)f)) & 15) == 0;
 }
@@ -360,6 +466,24 @@ int ln_bwd_grid(int M, int C) {
   return g < most ? g : most;
 }
 
+// One launch (ea_ln_bwd_few_kernel)?  us, one launch / two: 1 x 1280 2.5 / 6.7, 512 x 1280 3.7 / 8.5, 616 x 1024 in 8 bits 4.2 / 8.5, 1024 x 1280
+// 5.5 / 8.7, 1024 x 4096 10.9 / 19.8, 2048 x 1280 12.6 / 12.1, 4096 x 1280 24.6 / 13.9; the width decides little.  (Rows that start anywhere: 512 x
+// 777 7.4 / 9.8, 1024 x 777 13.1 / 10.1, where the second launch's 3.4 us on the host make up for it.)
+bool ln_bwd_few(int M) {
+  const int v = ea_forced_variant();       // tests: 101 pins the one launch, 102 the two
+  return v == 101 || (v != 102 && M <= 1024);
+}
+
+template <int XK, bool F32, bool ANY>
+int ln_bwd_few_launch(const LnBwdParams& p, float* dgamma, float* dbeta, void* stream) {
+  const int lpr = ln_lanes(p.C), rows = 4 * (64 / lpr), ncol = (p.C + LF_COLS - 1) / LF_COLS;
+  auto k = lpr == 16 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 16, 3> : lpr == 32 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 32, 3>
+         : p.C <= 1536 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 3> : p.C <= 2560 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 5>
+         : ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 8>;
+  EA_LAUNCH(k, dim3(ncol + (p.M + rows - 1) / rows), dim3(256), LF_LDS, stream, p, dgamma, dbeta, ncol);
+  return ea_launch_status();
+}
+
 template <int XK, bool F32, bool ANY>
 int ln_bwd_launch(const LnBwdParams& p, int grid, void* stream) {
   const int lpr = ln_lanes(p.C), smem = 4 * p.C * (int)sizeof(float);
@@ -371,7 +495,8 @@ int ln_bwd_launch(const LnBwdParams& p, int grid, void* stream) {
   return ea_launch_status();
 }
 template <int XK, bool F32>
-int ln_bwd_pick(const LnBwdParams& p, bool vec, int grid, void* stream) {
+int ln_bwd_pick(const LnBwdParams& p, bool vec, int grid, float* dgamma, float* dbeta, void* stream) {
+  if (!grid) return vec ? ln_bwd_few_launch<XK, F32, false>(p, dgamma, dbeta, stream) : ln_bwd_few_launch<XK, F32, true>(p, dgamma, dbeta, stream);
   return vec ? ln_bwd_launch<XK, F32, false>(p, grid, stream) : ln_bwd_launch<XK, F32, true>(p, grid, stream);
 }
 
@@ -390,28 +515,30 @@ extern "C" int ea_layernorm_train(const void* x, int in_f32, const float* gamma,
 }
 
 extern "C" size_t ea_layernorm_bwd_workspace_bytes(int M, int C) {
-  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096) return 0;
+  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096 || ln_bwd_few(M)) return 0;
   return (size_t)ln_bwd_grid(M, C) * 2 * C * sizeof(float);
 }
 
 extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const unsigned char* x_scale, const float* stats,
                                 const float* gamma, const void* residual, void* dx, float* dgamma, float* dbeta, int M, int C,
                                 void* workspace, size_t ws_bytes, void* stream) {
-  if (!dy || !x || !stats || !gamma || !dx || !dgamma || !dbeta || !workspace || (x_kind == XK_FP8 && !x_scale)) return EA_ERR_BAD_ARG;
+  if (!dy || !x || !stats || !gamma || !dx || !dgamma || !dbeta || (x_kind == XK_FP8 && !x_scale)) return EA_ERR_BAD_ARG;
   if (x_kind < XK_F16 || x_kind > XK_FP8) return EA_ERR_BAD_ARG;
   if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)stats & 7) || ((uintptr_t)workspace & 3)) return EA_ERR_BAD_ARG;
-  if (ws_bytes < ea_layernorm_bwd_workspace_bytes(M, C)) return EA_ERR_WORKSPACE;
+  const bool few = ln_bwd_few(M);
+  if (!few && (!workspace || ws_bytes < ea_layernorm_bwd_workspace_bytes(M, C))) return EA_ERR_WORKSPACE;
   LnBwdParams p;
   p.dy = (const f16*)dy; p.x = x; p.x_scale = x_scale; p.stats = stats; p.gamma = gamma; p.residual = residual; p.dx = dx;
   p.part = (float*)workspace; p.M = M; p.C = C;
   p.xpitch = x_kind == XK_FP8 ? ea_fp8_blocks(C) * EA_FP8_BLOCK : C;
   p.xspitch = ea_fp8_scale_pitch(M);
   const bool vec = ln_vec(C, dy, x, gamma, residual, dx, nullptr);
-  const int grid = ln_bwd_grid(M, C);
-  const int st = x_kind == XK_F16 ? ln_bwd_pick<XK_F16, false>(p, vec, grid, stream)
-               : x_kind == XK_F32 ? ln_bwd_pick<XK_F32, true>(p, vec, grid, stream) : ln_bwd_pick<XK_FP8, false>(p, vec, grid, stream);
-  if (st != EA_OK) return st;
+  const int grid = few ? 0 : ln_bwd_grid(M, C);
+  const int st = x_kind == XK_F16 ? ln_bwd_pick<XK_F16, false>(p, vec, grid, dgamma, dbeta, stream)
+               : x_kind == XK_F32 ? ln_bwd_pick<XK_F32, true>(p, vec, grid, dgamma, dbeta, stream)
+                                  : ln_bwd_pick<XK_FP8, false>(p, vec, grid, dgamma, dbeta, stream);
+  if (st != EA_OK || few) return st;
   auto k = ea_ln_join_kernel;
   EA_LAUNCH(k, dim3((2 * C + 31) / 32), dim3(1024), 32 * 33 * sizeof(float), stream, (const float*)workspace, dgamma, dbeta, grid, C);
   return ea_launch_status();

@@ -1203,9 +1203,9 @@ def layernorm_backward(dy, x, stats, gamma, residual=None):
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
     lib = _lib()
     nbytes = lib.ea_layernorm_bwd_workspace_bytes(M, Cc)
-    ws = torch.empty_strided((nbytes,), (1,), dtype=_U8, device=dev)
+    ws = torch.empty_strided((nbytes,), (1,), dtype=_U8, device=dev) if nbytes else None
     _run(dev, "ea_layernorm_bwd", lib.ea_layernorm_bwd, dy.data_ptr(), xt.data_ptr(), kind, x.scale.data_ptr() if q8 else None, stats.data_ptr(),
-         gamma.data_ptr(), _p(residual), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), M, Cc, ws.data_ptr(), nbytes)
+         gamma.data_ptr(), _p(residual), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), M, Cc, _p(ws), nbytes)
     return dx, dgamma, dbeta
 
 

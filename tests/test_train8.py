@@ -282,7 +282,7 @@ def ln_stats(x, eps):
 
 
 LN_SHAPES = [(1, 1), (1, 8), (5, 320), (70, 320), (9, 384), (6, 392), (37, 640), (5, 1280), (3, 1288), (2, 2560), (3, 2568), (2, 4096), (3, 77),
-             (5, 513), (2, 1537), (2, 4095)]
+             (5, 513), (2, 1537), (2, 4095), (521, 40)]
 
 
 @pytest.mark.parametrize("fp8", [0, 1])
@@ -321,9 +321,11 @@ def test_layernorm_train(kb, M, C, in_f32, fp8):
         assert (kb.down(y)[M] == 7).all()
 
 
+@pytest.mark.parametrize("launches", [1, 2])
 @pytest.mark.parametrize("kind,res", [(0, 0), (0, 1), (1, 0), (1, 1), (2, 0), (2, 1)])
 @pytest.mark.parametrize("M,C", LN_SHAPES)
-def test_layernorm_backward(kb, M, C, kind, res):
+def test_layernorm_backward(kb, M, C, kind, res, launches):
+    force(kb, 100 + launches)
     x = rows(9, M, C, np.float32 if kind else np.float16)
     gn = np.random.default_rng(10)
     gamma = (1 + 0.3 * gn.standard_normal(C)).astype(np.float32)
@@ -338,10 +340,13 @@ def test_layernorm_backward(kb, M, C, kind, res):
         x, xs, x64 = q, pack_scales(e), values(q, e, C)
     st = np.stack([mu, r], 1).astype(np.float32)
     dx, dg, db = kb.up(np.full((M + 1, C), 7, out)), kb.zeros((C,), np.float32), kb.zeros((C,), np.float32)
-    ws = kb.zeros((kb.lib.ea_layernorm_bwd_workspace_bytes(M, C) // 4,), np.float32)
-    args = (ptr(dy), ptr(x), kind, ptr(xs), ptr(st), ptr(gamma), ptr(residual), ptr(dx), ptr(dg), ptr(db), M, C, ptr(ws))
-    assert kb.lib.ea_layernorm_bwd(*args, ws.nbytes - 1 if kb.name == "emu" else ws.numel() * 4 - 1, kb.stream) == -4
-    assert kb.lib.ea_layernorm_bwd(*args, ws.nbytes if kb.name == "emu" else ws.numel() * 4, kb.stream) == 0
+    nbytes = kb.lib.ea_layernorm_bwd_workspace_bytes(M, C)
+    assert (nbytes > 0) == (launches == 2)
+    ws = kb.zeros((nbytes // 4,), np.float32) if nbytes else None
+    args = (ptr(dy), ptr(x), kind, ptr(xs), ptr(st), ptr(gamma), ptr(residual), ptr(dx), ptr(dg), ptr(db), M, C)
+    if nbytes:
+        assert kb.lib.ea_layernorm_bwd(*args, ptr(ws), nbytes - 1, kb.stream) == kb.lib.ea_layernorm_bwd(*args, None, nbytes, kb.stream) == -4
+    assert kb.lib.ea_layernorm_bwd(*args, ptr(ws), nbytes, kb.stream) == 0
     mu, r = st.astype(np.float64).T
     n = (x64 - mu[:, None]) * r[:, None]
     d = dy.astype(np.float64)
@@ -600,7 +605,7 @@ def test_the_c_entries_refuse(emu_lib):
     assert lib.ea_layernorm_bwd(p, p, 3, None, p, p, None, o, o, o, 1, 8, p, 1 << 20, None) == -2
     assert lib.ea_layernorm_bwd(p, p, 2, None, p, p, None, o, o, o, 1, 8, p, 1 << 20, None) == -2
     assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, o, o, 1, 5000, p, 1 << 20, None) == -1
-    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, o, o, 1, 8, p, 0, None) == -4
+    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, o, o, 4096, 8, p, 0, None) == -4
     assert lib.ea_layernorm_bwd_workspace_bytes(0, 8) == 0 and lib.ea_layernorm_bwd_workspace_bytes(1, 4097) == 0
     e = epilogue(a)
     g = lambda **kw: lib.ea_gemm_fp8(kw.get("a", p), kw.get("sa", p), p, p, kw.get("M", 16), kw.get("N", 16), kw.get("K", 128),  # noqa: E731

@@ -279,15 +279,15 @@ __device__ __forceinline__ f16 wl_factor(int byte) {
   return __builtin_bit_cast(f16, u);
 }
 
-// A lane's share of db: the 8 rows that a dy fragment holds of its column.  On the vector unit, beside the products: summed by the matrix
-// unit with a row of ones, two fragments in one accumulator, the zeros of one's operand times an infinity of the other's column made NaN.
-__device__ __forceinline__ void wl_sum8(float& s, f16x8 v) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) s += (float)v[j];
-}
-__device__ __forceinline__ float wl_sum_rows(float s) {     // lanes l15, + 16, + 32, + 48 hold the other rows of the column
-  s += ea_shfl_xor(s, 16);
-  return s + ea_shfl_xor(s, 32);
+// an MFMA operand of ones: every row of the product is the column sums of the other operand.  One accumulator per fragment: where two
+// fragments shared one (each with a single row of ones), the zeros times an infinity of one's column made NaN of the other's sum.  On
+// the vector unit the sums cost 3 % of 8192^3 and 5 % of 616 x 1280 x 1024.
+__device__ __forceinline__ f16x8 wl_ones() {
+  unsigned u = 0x3c003c00u;
+#ifndef EA_EMU
+  asm volatile("" : "+v"(u));              // (made where it is used: kept over the loop, its four registers were spilled)
+#endif
+  return __builtin_bit_cast(f16x8, u32x4{u, u, u, u});
 }
 
 // ------------------------------------------------------------------------------------- weight gradient, 128 x 128 tiles
@@ -330,8 +330,7 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
     ad[i] = r * 256 + (((wm * 4 + (i ^ (2 * wn))) ^ wl_dy_swz(r)) << 5) + (l15 & 3) * 8;
     ax[i] = WR_DY + s * 128 + (((wn * 4 + i) ^ wl_x_swz(s)) << 4) + (l15 & 1) * 8;
   }
-  f32x4 acc[4][4];
-  float colsum[2] = {0.0f, 0.0f};
+  f32x4 acc[4][4], accb[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -380,8 +379,8 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][j] = ea_mfma_16x16x32(fx[j][ks], fa[i][ks], acc[i][j]);
         if (sums) {
-          wl_sum8(colsum[0], fa[0][ks]);
-          wl_sum8(colsum[1], fa[1][ks]);
+          accb[0] = ea_mfma_16x16x32(wl_ones(), fa[0][ks], accb[0]);
+          accb[1] = ea_mfma_16x16x32(wl_ones(), fa[1][ks], accb[1]);
         }
       }
     }
@@ -391,11 +390,8 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
 #pragma unroll
   for (int i = 0; i < 4; ++i) {            // D^T: a lane holds 4 consecutive k of one n
     const int n = n0 + wm * 64 + (i ^ (2 * wn)) * 16 + l15;
-    if (i < 2 && sums) {
-      const float t = wl_sum_rows(colsum[i & 1]);
-      if (n < p.N && lq == 0) db[n] = t;
-    }
     if (n >= p.N) continue;
+    if (i < 2 && sums && lq == 0) db[n] = accb[i & 1][0];
 #pragma unroll
     for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wn * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
   }
@@ -453,8 +449,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
   };
   auto stage_x = [&](int h) { wl_dma16(rx, vx[h] + ox, sbuf + WL_DY + h * 8192 + wave * 1024); };
 
-  f32x4 acc[8][4];
-  float colsum[2] = {0.0f, 0.0f};       // of quadrants 0 and 1
+  f32x4 acc[8][4], accb = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -502,13 +497,13 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[qa * 4 + i][qb * 2 + j] = ea_mfma_16x16x32(fb[j][ks], fa[i][ks], acc[qa * 4 + i][qb * 2 + j]);
-      if (sums) wl_sum8(colsum[qa], fa[0][ks]);
+      if (sums) accb = ea_mfma_16x16x32(wl_ones(), fa[0][ks], accb);
     }
 #ifndef EA_EMU
     __builtin_amdgcn_s_setprio(0);
 #endif
   };
-  const bool sums = tk == 0;
+  // dy's column sums, one accumulator's worth per workgroup: quadrants 0 by the first k tile, 1 by the second (there are two: wgrad_plan)
   auto body = [&](int t, auto more_c) {
     constexpr bool more = decltype(more_c)::value;
     const char* buf = smem + (t & 1) * WL_STEP;
@@ -516,7 +511,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
     read_d(buf, c0);
     if (more) ea_wait_dma<2>(); else ea_wait_dma<0>();
     ea_f8l_barrier();
-    mma(c0, c0, fb0, sums);
+    mma(c0, c0, fb0, tk == 0);
     ea_f8l_barrier();
     if (more) stage_d(0);
     read_x(t, c1, fb1);
@@ -528,7 +523,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
     read_d(buf, c1);
     if (more) ea_wait_dma<4>();
     ea_f8l_barrier();
-    mma(c1, c1, fb1, sums);
+    mma(c1, c1, fb1, tk == 1);
     ea_f8l_barrier();
     if (more) {
       read_x(t + 1, c0, fbn);
@@ -580,13 +575,10 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
 #pragma unroll
     for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wn * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
   }
-  if (sums)
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int n = n0 + wm * 128 + q * 64 + wn * 16 + l15;
-      const float t = wl_sum_rows(colsum[q]);
-      if (n < p.N && lq == 0) db[n] = t;
-    }
+  if (tk < 2 && lq == 0) {
+    const int n = n0 + wm * 128 + tk * 64 + wn * 16 + l15;
+    if (n < p.N) db[n] = accb[0];
+  }
 }
 
 // sum of the slices, in their order
@@ -612,12 +604,13 @@ struct WgradPlan { int kernel, splits, rows; };
 WgradPlan wgrad_plan(int M, int N, int K) {
   WgradPlan w{-1, 1, 64};
   const int v = ea_forced_variant();       // tests: 101, 102, 103 pin a kernel
+  const bool large = K > 256;              // (two k tiles: each sums one half of its dy columns for db)
   const bool dma = (N & 7) == 0 && N <= (1 << 18) && K <= (1 << 18) && v != 103;
   const double nk = (double)N * K;
   const int steps = (M + 63) / 64;
   double best = 0;
   for (int kernel = 256; kernel >= 0; kernel -= 128) {
-    if (kernel ? !dma || (v == 101 && kernel != 256) || (v == 102 && kernel != 128) : dma) continue;
+    if (kernel ? !dma || (kernel == 256 ? !large || v == 102 : large && v == 101) : dma) continue;
     const int tile = kernel == 256 ? 256 : 128;
     const long long tiles = (long long)((N + tile - 1) / tile) * ((K + tile - 1) / tile);
     for (int s = 1; s <= steps && s <= 64; ++s) {

@@ -15,7 +15,7 @@ namespace {
 // become infinite.
 // Both operands have the contracted axis as their ROW axis, so they go to LDS row-major and the fragments are read transposed: 16 lanes
 // take a 4 x 16 (fp16) or 8 x 16 (codes) block and each ends up with consecutive rows of one column.  Bound by the matrix unit at
-// the fp16 rate: 8192^3 915 us = 1200 TFLOP/s (the library's fp16 product: 1382).
+// the fp16 rate: 8192^3 905 us = 1215 TFLOP/s (the library's fp16 product: 1382).
 // First the kernel for any N and alignment: 128 x 128 tiles, both operands through registers, x decoded on the way to LDS.
 struct WgradParams {
   const f16* dy; const uint8_t* x; const uint8_t* sx;
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(64) void ea_fp8_wgrad_join_kernel(const float* part
 // Kernel (256, 128: the DMA kernels; 0: the one for any N and alignment) and number of slices of the rows: the least time by a model of
 // what was measured.  A 64-row step takes a 256 x 256 workgroup 1.65 us, a 128 x 128 one 0.87 us alone on its CU and 1.25 us beside
 // another; a workgroup's start and end 10 / 5 us; joining s slices 4 us and 2 s + 1 passes over the output at 8 TB/s.
-//   16384 x 1280 x 5120 (M x N x K): 256 with 5 slices 220 us (2: 225, 1: 400; 128: 263 at best), 32768 x 2560 x 320: 256 with 12 slices 89
+//   16384 x 1280 x 5120 (M x N x K): 256 with 5 slices 216 us (2: 225, 1: 400; 128: 263 at best), 32768 x 2560 x 320: 256 with 12 slices 89
 //   (128 with 8: 103), 8192 x 640 x 640: 128 with 10 slices 25 (1: 111; 256 with 24: 32), 616 x 1280 x 1024: 128 with 1 slice 14 (2: 19; 256: 27)
 // Workspace and launch go by the same answer, which depends on the sizes alone.
 struct WgradPlan { int kernel, splits, rows; };
@@ -652,13 +652,13 @@ int fp8_large_launch(const EaFp8GemmParams& p, void* stream) {
 
 // Which kernel (times in us on the MI355X, M x N x K):
 //   256 x 256 tiles, one workgroup per CU: from 8 K tiles on, where the last round of 256 workgroups is at least as full as three
-//       quarters of all rounds.  16384 x 5120 x 1280 115 (128 x 128: 126), 8192^3 391 (504); 16384 x 1280 x 5120 fills 1.25 rounds:
-//       123 (115), and 5 K tiles do not carry the larger tile's start and end: 8192 x 5120 x 640 62 (57)
-//   128 x 128, two workgroups per CU (one multiplies while the other starts or stores): from 256 tiles on.  32768 x 320 x 320 17.0
-//       (64 x 128: 16.1, 64 x 64: 22.7), 16384 x 5120 x 1280 126 (154, 231)
-//   64 x 128: from 160 tiles on.  616 x 2560 x 1024 6.6 (64 x 64: 7.3, 128 x 128: 8.5), 2048 x 1280 x 1280 9.9 (12.9, 9.9)
-//   64 x 64 with a ring of four: few tiles, where each K tile's latency counts.  512 x 1280 x 5120 15.8 (64 x 128: 24.1),
-//       77 x 1024 x 1024 5.7 (5.9)
+//       quarters of all rounds.  16384 x 5120 x 1280 113 (128 x 128: 125), 8192^3 383 (492); 16384 x 1280 x 5120 fills 1.25 rounds:
+//       111.5 (110.5), and 5 K tiles do not carry the larger tile's start and end: 8192 x 5120 x 640 45.4 (43.4)
+//   128 x 128, two workgroups per CU (one multiplies while the other starts or stores): from 256 tiles on.  32768 x 320 x 320 12.8
+//       (64 x 128: 14.1, 64 x 64: 21.1), 16384 x 5120 x 1280 125 (150, 234)
+//   64 x 128: from 160 tiles on.  616 x 2560 x 1024 6.7 (64 x 64: 7.5, 128 x 128: 8.5), 2048 x 1280 x 1280 9.9 (13.2, 10.0)
+//   64 x 64 with a ring of four: few tiles, where each K tile's latency counts.  512 x 1280 x 5120 15.4 (64 x 128: 23.1),
+//       77 x 1024 x 1024 6.1 (6.0)
 int fp8_launch(EaFp8GemmParams& p, void* stream) {
   p.raster_gm = 8;                         // (4 and 16: within 2 %)
   const int v = ea_forced_variant();

@@ -143,7 +143,8 @@ typedef struct ea_tuning {
   int32_t variant;             /* 0 auto, k: force instantiation k of the LDS-DMA kernels (1 / 9: ea_gemm2.h 128- / 64-row tiles,
                                   30: ea_gemm8.h 256 x 256 tiles, 33 / 34: the 64- / 128-row tiles with a 3-stage ring -- two K tiles in flight, for
                                   weights that come from HBM; 101 ... 104: ea_gemm_fp8's 256 x 256, 128 x 128, 64 x 128 and
-                                  64 x 64 tiles; the rest: tools builds) */
+                                  64 x 64 tiles, 101 ... 103: ea_gemm_fp8_wgrad's 256-, 128-column and any-N kernels, 101 / 102:
+                                  ea_layernorm_bwd in one / two launches; the rest: tools builds) */
   int32_t splits;              /* 0 plan's own, s: force the split-K factor */
   int32_t bn;                  /* 0 plan's own, 128: force 128-wide column tiles */
   int32_t no_register_direct;  /* 1: LDS-slab epilogue where the register-direct one would run */

@@ -1260,6 +1260,10 @@ def gemm_fp8(a, w, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=t
             and (out is None or (out.dtype in (_F16, _F32) and out.shape == shape))):
         _refuse(f"gemm_fp8: bias must be fp32 [{N}], residual and out fp16 or fp32 {shape}", bias=bias, residual=residual, out=out,
                 out_dtype=out_dtype)
+    if out is not None and residual is not None:
+        po, pr = out.data_ptr(), residual.data_ptr()
+        if (po != pr or out.dtype != residual.dtype) and po < pr + residual.nbytes and pr < po + out.nbytes:
+            _refuse("gemm_fp8: residual has to be out or lie apart from it", residual=residual, out=out)
     _on_device(dev, a.q, a.scale, w.q, w.scale, bias, residual, out)
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=dev)

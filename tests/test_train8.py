@@ -670,6 +670,18 @@ def test_the_public_functions_refuse():
             f()
 
 
+def test_gemm_fp8_refuses_a_residual_that_overlaps_the_output():
+    t = ops.Fp8Tensor(torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(1, 16, dtype=torch.uint8), 8)
+    w = ops.Fp8Tensor(torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(1, 1, dtype=torch.uint8), 8)
+    buf = torch.zeros(8, 4)
+    for out, res in ((buf[:4], buf[1:5]), (buf[3:7], buf[:4]), (buf[:4], buf.view(torch.float16).view(16, 4)[:4])):
+        with pytest.raises(ValueError, match="apart"):
+            ops.gemm_fp8(t, w, out=out, residual=res)
+    for out, res in ((buf[:4], buf[:4]), (buf[:4], buf[4:])):       # accepted: on the CPU only the missing device stops them
+        with pytest.raises(RuntimeError, match="MI355X"):
+            ops.gemm_fp8(t, w, out=out, residual=res)
+
+
 # --------------------------------------------------------------------------------------------------------- capturing, on the CPU
 def test_no_garbage_collection_inside_a_capture(monkeypatch):
     """A dead cycle is not collected while any thread captures, and collection is as it was afterwards, also behind errors."""

@@ -92,6 +92,14 @@ __device__ __forceinline__ u32x4 ea_rows_load(ea_rows r, unsigned off) {
 __device__ __forceinline__ void ea_rows_store(ea_rows r, unsigned off, u32x4 v) {
   if (off < r.n && off + 16 <= r.n) memcpy(r.p + off, &v, 16);
 }
+__device__ __forceinline__ unsigned ea_rows_load1(ea_rows r, unsigned off) {
+  unsigned v = 0;
+  if (off < r.n && off + 4 <= r.n) memcpy(&v, r.p + off, 4);
+  return v;
+}
+__device__ __forceinline__ void ea_rows_store1(ea_rows r, unsigned off, unsigned v) {
+  if (off < r.n && off + 4 <= r.n) memcpy(r.p + off, &v, 4);
+}
 #else
 typedef __amdgpu_buffer_rsrc_t ea_rows;
 __device__ __forceinline__ ea_rows ea_make_rows(const void* p, long long bytes) {
@@ -103,6 +111,8 @@ __device__ __forceinline__ u32x4 ea_rows_load(ea_rows r, unsigned off) {
 __device__ __forceinline__ void ea_rows_store(ea_rows r, unsigned off, u32x4 v) {
   __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, 0);
 }
+__device__ __forceinline__ unsigned ea_rows_load1(ea_rows r, unsigned off) { return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0); }
+__device__ __forceinline__ void ea_rows_store1(ea_rows r, unsigned off, unsigned v) { __builtin_amdgcn_raw_buffer_store_b32(v, r, off, 0, 0); }
 #endif
 
 // acc[i][j] of one wave (16 x 16 fragments): activation fragments i (groups of FMG), weight fragments j (groups of FNG): a lane owns

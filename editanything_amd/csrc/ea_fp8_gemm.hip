@@ -2,17 +2,22 @@
 // ea_gemm_fp8_wgrad, the weight and bias gradient of a Linear from its 8-bit input.
 #include "ea_fp8_gemm.h"
 
-int ea_forced_variant();          // ea_gemm.hip: the calling thread's ea_tuning.variant (tests)
+int ea_forced_variant();          // ea_gemm.hip: the calling thread's ea_tuning.variant and .splits (tests)
+int ea_forced_splits();
 
 namespace {
 
 // ---------------------------------------------------------------------------------------------------- weight gradient
 //   dw[n][k] = sum_m dy[m][n] x[m][k],  x[m][k] = code * 2^E[m][k / 128];     db[n] = sum_m dy[m][n]
 // The sum runs over rows, and each row has its own exponents, so the matrix unit's block scales do not apply (they belong to runs of
-// the contracted axis).  x is decoded to fp16 instead -- four significant bits, exact -- and multiplied by dy as it is: every product
-// is exact, the sums are fp32.  x is decoded as x / 2 and the accumulators are doubled: e4m3 rounding can carry an fp16 maximum
-// (65504) to 65536, and at the small end x / 2 loses no more than fp16's own last step.  Blocks whose maximum exceeds 448 * 2^8 = 114688
-// become infinite.
+// the contracted axis).  x is decoded to fp16 instead and multiplied by dy as it is: every product is exact, the sums are fp32.
+// fp16 holds 40 octaves, the format 220, so x goes in as x / 2^U and the accumulators count in units of 2^U: a code times 2^f, f = E - U,
+// is an fp16 value for -15 <= f <= 7 (the code's smallest step 2^-9 times 2^-15 is fp16's, 448 * 2^7 is 57344).  U belongs to a block column
+// of 128 and is chosen for up to 2048 rows at a time (WxUnit): from the exponents of those rows, and where it changes, the accumulators are
+// multiplied by the power of two between.  Rows that do not fit one window of 23 octaves are taken in several passes over the same rows, each with
+// the others' factors 0 (a block of zeros has E = 0, so padding rows among tiny ones do that).  Choosing a unit costs 0.6 us per 2048 rows: the
+// scale bytes' extremes are joined over the workgroup before the first factor can be written (616 x 1280 x 1024 13.8 -> 14.4 us, 16384 x 1280 x 5120
+// 218 -> 225).
 // Both operands have the contracted axis as their ROW axis, so they go to LDS row-major and the fragments are read transposed: 16 lanes
 // take a 4 x 16 (fp16) or 8 x 16 (codes) block and each ends up with consecutive rows of one column.  Bound by the matrix unit at
 // the fp16 rate: 8192^3 905 us = 1215 TFLOP/s (the library's fp16 product: 1382).
@@ -26,6 +31,7 @@ struct WgradParams {
 
 constexpr int WG_T = 128, WG_R = 64;                     // tile columns of n and of k, rows per step
 constexpr int WG_BUF = WG_R * WG_T * 2;                  // one operand's tile: 16 KiB
+constexpr int WG_CH = 32 * WG_R, WG_LDS = 2 * WG_BUF + 16;      // rows under one choice of the unit; the tiles and the waves' extremes
 // byte of (row, column) in a tile
 __device__ __forceinline__ int wg_at(int r, int c) { return r * 256 + ((((c >> 4) ^ r) & 7) << 5) + (c & 15) * 2; }
 
@@ -47,6 +53,65 @@ __device__ __forceinline__ f16x8 wg_frag(const char* buf, int r0, int c0, int la
   return f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
+// The unit 2^(u - 127) of the accumulators of one block column and the exponent bytes that are still to be taken of the rows at hand.
+// Accumulators are below 2^62 units (2^30 rows of |dy| 65504 times 57344) and worth keeping from 2^-72 on (2^-24 of the smallest product, 2^-24
+// times 2^-24), so within WX_REACH octaves a change of units neither overflows fp32 nor loses anything in its subnormal numbers; a wider one adds the
+// sums to the output and starts them anew.
+constexpr int WX_NONE = -1000, WX_REACH = 50;
+struct WxUnit {
+  int u = WX_NONE, bottom = 0, top = 0, lo = 0, hi = -1;
+  // The next pass: the unit becomes u, its rows have the bytes from ... to (none: from > to).  Returns true where the sums, still in
+  // units of `old`, have to be put away first
+  __device__ __forceinline__ bool next(int& from, int& to, int& old) {
+    old = u;
+    from = lo;
+    to = hi;
+    if (hi < lo) return false;
+    if (hi - u > 7 || lo - u < -15) {
+      if (hi - 22 > from) from = hi - 22;
+      u = hi - 7;
+    }
+    hi = from - 1;
+    const int b = u < bottom ? u : bottom, t = u > top ? u : top;
+    const bool first = old == WX_NONE, away = !first && t - b > WX_REACH;
+    bottom = first || away ? u : b;
+    top = first || away ? u : t;
+    if (first) old = u;
+    return away;
+  }
+};
+// Extremes of the bytes of some rows: (hi, 255 - lo) in the halves of a word, whose maximum is taken for both at once
+__device__ __forceinline__ unsigned wx_max(unsigned a, unsigned b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ unsigned wx_word(int byte) { return (unsigned)byte | (unsigned)(255 - byte) << 16; }
+// each wave's word to red[wave]; after a barrier the words of waves first, first + step, ... are joined
+__device__ __forceinline__ void wx_range_put(unsigned* red, unsigned w) {
+  w = ea_f2u(ea_group_reduce<64>(ea_u2f(w), [](float a, float b) { return ea_u2f(wx_max(ea_f2u(a), ea_f2u(b))); }));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = w;
+}
+template <int FIRST, int STEP, int WAVES>
+__device__ __forceinline__ void wx_range_get(const unsigned* red, WxUnit& x) {
+  unsigned w = red[FIRST];
+#pragma unroll
+  for (int i = FIRST + STEP; i < WAVES; i += STEP) w = wx_max(w, red[i]);
+  w = (unsigned)ea_uniform((int)w);
+  x.hi = (int)(w & 0xffff);
+  x.lo = 255 - (int)(w >> 16);
+}
+// acc *= 2^d, or = 0
+template <int I, int J>
+__device__ __forceinline__ void wx_rescale(f32x4 (&acc)[I][J], bool zero, int d) {
+  if (!zero && d == 0) return;
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = zero ? 0.0f : ldexpf(acc[i][j][r], d);
+}
+
 __device__ __forceinline__ void wg_decode16(u32x4 w, float s, f16x8& a, f16x8& b) {
   float v[16];
 #pragma unroll
@@ -55,14 +120,41 @@ __device__ __forceinline__ void wg_decode16(u32x4 w, float s, f16x8& a, f16x8& b
   for (int j = 0; j < 8; ++j) { a[j] = (f16)(v[j] * s); b[j] = (f16)(v[8 + j] * s); }
 }
 
-// doubled accumulators to row[k ... k + 3]
-__device__ __forceinline__ void wg_store4(float* row, int k, int K, f32x4 v) {
+// Accumulators in units of 2^(u - 127) to dw, or added to it: fragment (i, j) holds the 4 columns k + 16 j of row row(i) + l of the tile (D^T: a
+// lane has 4 consecutive k of one n).  `out` starts at the tile's first row and ends with the matrix; columns that are not there lie 2 GiB on.
+template <int I, int J, typename F>
+__device__ __forceinline__ void wg_put(ea_rows out, const f32x4 (&acc)[I][J], F row, int l, int k, int K, int u, bool add) {
+#ifndef EA_EMU
+  asm volatile("" : "+v"(l), "+v"(k));     // (the offsets are made here: over the loop they would take the accumulators' registers)
+#endif
   if ((K & 3) == 0) {
-    if (k < K) *reinterpret_cast<f32x4*>(row + k) = v * 2.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const unsigned c = k + 16 * j < K ? (unsigned)(k + 16 * j) * 4u : EA_F8_NOWHERE;
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const unsigned o = c + (unsigned)(row(i) + l) * (unsigned)K * 4u;
+        f32x4 v = acc[i][j];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], u - 127);
+        if (add) v += __builtin_bit_cast(f32x4, ea_rows_load(out, o));
+        ea_rows_store(out, o, __builtin_bit_cast(u32x4, v));
+      }
+    }
   } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (k + r < K) row[k + r] = v[r] * 2.0f;
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const unsigned c = k + 16 * j + r < K ? (unsigned)(k + 16 * j + r) * 4u : EA_F8_NOWHERE;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+          const unsigned o = c + (unsigned)(row(i) + l) * (unsigned)K * 4u;
+          float v = ldexpf(acc[i][j][r], u - 127);
+          if (add) v += ea_u2f(ea_rows_load1(out, o));
+          ea_rows_store1(out, o, ea_f2u(v));
+        }
+      }
   }
 }
 
@@ -77,6 +169,8 @@ __global__ __launch_bounds__(256) void ea_fp8_wgrad_kernel(WgradParams p) {
   u32x4 xr[2];
   float xs[2];
   f16x8 dr[4];
+  WxUnit unit;
+  int from = 0, to = 0;
   auto load = [&](int m0) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -84,7 +178,8 @@ __global__ __launch_bounds__(256) void ea_fp8_wgrad_kernel(WgradParams p) {
       const bool ok = m < m_end;
       const long long mm = ok ? m : m_begin;
       xr[i] = *reinterpret_cast<const u32x4*>(p.x + mm * p.Kp + k0 + c);
-      xs[i] = ok ? ea_fp8_scale(p.sx[(long long)tk * p.Rp + mm]) * 0.5f : 0.0f;
+      const int b = p.sx[(long long)tk * p.Rp + mm];
+      xs[i] = ok && b >= from && b <= to ? ldexpf(1.0f, b - unit.u) : 0.0f;
       if (!ok) xr[i] = u32x4{0, 0, 0, 0};                  // (a NaN code must not reach the sum)
     }
 #pragma unroll
@@ -126,39 +221,68 @@ __global__ __launch_bounds__(256) void ea_fp8_wgrad_kernel(WgradParams p) {
   f16x8 ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = (f16)1.0f;
-  if (m_begin < m_end) load(m_begin);
-  for (int m0 = m_begin; m0 < m_end; m0 += WG_R) {
-    __syncthreads();
-    store();
-    __syncthreads();
-    if (m0 + WG_R < m_end) load(m0 + WG_R);
-#pragma unroll
-    for (int h = 0; h < WG_R; h += 32) {
-      f16x8 fd[4], fx[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) fd[i] = wg_frag(smem, h, wn * 64 + i * 16, lane);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) fx[j] = wg_frag(smem + WG_BUF, h, wk * 64 + j * 16, lane);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = ea_mfma_16x16x32(fx[j], fd[i], acc[i][j]);
-      if (tk == 0 && wk == 0)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) accb[i] = ea_mfma_16x16x32(ones, fd[i], accb[i]);
-    }
-  }
-  float* dw = p.dw + (long long)blockIdx.y * p.part;
-  float* db = p.splits > 1 ? dw + (long long)p.N * p.K : p.db;
+  unsigned* const red = reinterpret_cast<unsigned*>(smem + 2 * WG_BUF);
+  float* const dw = p.dw + (long long)blockIdx.y * p.part;
+  const ea_rows out = ea_make_rows(dw + (long long)n0 * p.K, (long long)(p.N - n0) * p.K * 4);
   const int l15 = lane & 15, lq = lane >> 4;
+  bool stored = false;
+  auto put = [&](int u) {
+    wg_put(out, acc, [&](int i) { return wn * 64 + i * 16; }, l15, k0 + wk * 64 + 4 * lq, p.K, u, stored);
+    stored = true;
+  };
+  bool again = false;                      // another pass over the same rows
+  for (int c0 = m_begin;;) {
+    const bool end = c0 >= m_end;
+    const int c1 = m_end - c0 < WG_CH ? m_end : c0 + WG_CH;
+    if (!end && !again) {
+      unsigned w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {            // D^T: a lane holds 4 consecutive k of one n
-    const int n = n0 + wn * 64 + i * 16 + l15;
-    if (n >= p.N) continue;
+      for (int u = 0; u < WG_CH / 256; ++u) {
+        const int m = c0 + u * 256 + tid;
+        w = wx_max(w, wx_word(p.sx[(long long)tk * p.Rp + (m < c1 ? m : c0)]));      // (the first row once more changes nothing)
+      }
+      wx_range_put(red, w);
+      __syncthreads();
+      wx_range_get<0, 1, 4>(red, unit);
+    }
+    int old;
+    const bool away = unit.next(from, to, old);
+    if (end || away) put(old);
+    if (end) break;
+    wx_rescale(acc, away, old - unit.u);
+    const bool sums = tk == 0 && wk == 0 && !again;
+    load(c0);
+    for (int m0 = c0; m0 < c1; m0 += WG_R) {
+      __syncthreads();
+      store();
+      __syncthreads();
+      if (m0 + WG_R < c1) load(m0 + WG_R);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wk * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
-    if (tk == 0 && wk == 0 && lq == 0) db[n] = accb[i][0];
+      for (int h = 0; h < WG_R; h += 32) {
+        f16x8 fd[4], fx[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fd[i] = wg_frag(smem, h, wn * 64 + i * 16, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fx[j] = wg_frag(smem + WG_BUF, h, wk * 64 + j * 16, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = ea_mfma_16x16x32(fx[j], fd[i], acc[i][j]);
+        if (sums)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) accb[i] = ea_mfma_16x16x32(ones, fd[i], accb[i]);
+      }
+    }
+    again = unit.lo <= unit.hi;
+    if (!again) c0 += WG_CH;
   }
+  float* db = p.splits > 1 ? dw + (long long)p.N * p.K : p.db;
+  if (tk == 0 && wk == 0 && lq == 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + wn * 64 + i * 16 + l15;
+      if (n < p.N) db[n] = accb[i][0];
+    }
 }
 
 // -------------------------------------------------------------------------------------------- weight gradient, large tiles
@@ -168,16 +292,15 @@ __global__ __launch_bounds__(256) void ea_fp8_wgrad_kernel(WgradParams p) {
 // Both operands go to LDS as they are.  dy: half h holds the 64-column quadrants h of both wave rows, rows of 256 bytes, read with
 // ds_read_b64_tr_b16; x: half h holds the 32-column quadrants h of the four wave columns, rows of 128 bytes of CODES, read with
 // ds_read_b64_tr_b8: 16 lanes take 8 rows x 16 bytes and each gets 8 rows of one column.  The codes become fp16 in registers,
-//     x / 2 = (code 2^-8) * 2^(E + 7):   the conversion's own scale does the first factor, a packed fp16 product with the rows' 8 scale
-// factors (one 16-byte LDS read for 8 rows) the second; both are exact while x / 2 is an fp16 value.  E above 8 gives infinities, E below
-// -31 (|x| < 2^-23) zeros.
+//     x / 2^U = (code 2^-8) * 2^(E - U + 8):   the conversion's own scale does the first factor, a packed fp16 product with the rows' 8
+// scale factors (one 16-byte LDS read for 8 rows) the second; both are exact inside the unit's window.
 // The load parts: L0 reads dy quadrant 0, L1 reads and decodes x quadrant 1, L2 reads dy quadrant 1, L3 reads and decodes the next
 // step's x quadrant 0 (1.58 us per step with the chip two fifths full; decoding in the multiply parts
 // 1.71, spreading the dy reads over all four load parts 1.61).  DMA of the next step: x in L0, dy 0 in L1,
 // dy 1 in L2.  What L(q) issues is waited for in L(q + 2) (counted: the younger two parts' DMA stays in flight) and first read in
 // L(q + 3), one barrier after the lagging wave row's wait.
 constexpr int WL_DY = 32768, WL_X = 16384, WL_STEP = WL_DY + WL_X, WL_CH = 32;      // bytes per step; steps whose scale factors are in LDS
-constexpr int WL_SCL = 2 * WL_STEP, WL_LDS = WL_SCL + WL_CH * 2 * 64 * 2;
+constexpr int WL_SCL = 2 * WL_STEP, WL_RED = WL_SCL + WL_CH * 2 * 64 * 2, WL_LDS = WL_RED + 32;
 
 // 32-byte piece of a dy row, 16-byte piece of an x row: XORed so that the rows that a wave reads together cover the banks evenly
 __device__ __forceinline__ int wl_dy_swz(int r) { return (r & 3) | ((r >> 1) & 4); }
@@ -272,10 +395,10 @@ __device__ __forceinline__ f16x8 wl_decode8(u32x2 w, f16x8 s) {
   return __builtin_bit_cast(f16x8, h) * s;
 #endif
 }
-// 2^(E + 7) as fp16 from the stored byte E + 127
-__device__ __forceinline__ f16 wl_factor(int byte) {
-  const int e = byte - 120;
-  const unsigned short u = e >= 16 ? 0x7c00 : e >= -14 ? (unsigned short)((e + 15) << 10) : e >= -24 ? (unsigned short)(1 << (e + 24)) : 0;
+// 2^(E - U + 8) as fp16 from the stored byte (-7 ... 15 inside a window; less where the unit could not follow); 0 for a row of another pass
+__device__ __forceinline__ f16 wl_factor(int byte, int unit, int from, int to) {
+  const int e = byte - unit + 8;
+  const unsigned short u = byte < from || byte > to ? 0 : e >= -14 ? (unsigned short)((e + 15) << 10) : e >= -24 ? (unsigned short)(1 << (e + 24)) : 0;
   return __builtin_bit_cast(f16, u);
 }
 
@@ -293,7 +416,7 @@ __device__ __forceinline__ f16x8 wl_ones() {
 // ------------------------------------------------------------------------------------- weight gradient, 128 x 128 tiles
 // Few or small outputs: 4 waves (2 x 2) of 64 x 64, a ring of three 64-row steps (24 KiB each, two workgroups per CU), one barrier per
 // step; operands, fragment reads and decoding as in the large kernel.
-constexpr int WR_S = 3, WR_DY = 16384, WR_STEP = 24576, WR_CH = 32, WR_SCL = WR_S * WR_STEP, WR_LDS = WR_SCL + WR_CH * 64 * 2;
+constexpr int WR_S = 3, WR_DY = 16384, WR_STEP = 24576, WR_CH = 32, WR_SCL = WR_S * WR_STEP, WR_RED = WR_SCL + WR_CH * 64 * 2, WR_LDS = WR_RED + 16;
 __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p) {
   EA_SMEM(smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = ea_uniform(tid >> 6), wm = wave >> 1, wn = wave & 1;
@@ -335,24 +458,50 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const bool sums = tk == 0;
   char* const scl = smem + WR_SCL;
-  for (int t0 = 0; t0 < steps; t0 += WR_CH) {
+  unsigned* const red = reinterpret_cast<unsigned*>(smem + WR_RED);
+  WxUnit unit;
+  float* const dw = p.dw + (long long)blockIdx.y * p.part;
+  const ea_rows out = ea_make_rows(dw + (long long)n0 * p.K, (long long)(p.N - n0) * p.K * 4);
+  bool stored = false;
+  auto put = [&](int u) {
+    wg_put(out, acc, [&](int i) { return wm * 64 + (i ^ (2 * wn)) * 16; }, l15, k0 + wn * 64 + 4 * lq, p.K, u, stored);
+    stored = true;
+  };
+  bool again = false;                      // another pass over the same chunk
+  for (int t0 = 0;;) {
+    const bool end = t0 >= steps;
     const int n = steps - t0 < WR_CH ? steps - t0 : WR_CH;
     const long long mc = m_begin + t0 * 64ll;
-    if (t0) ea_raw_barrier();              // the chunk before this one has been read
-    const int left = (int)(m_end - mc);
-    const uint8_t* const sx = p.sx + tk * p.Rp + mc;
-    unsigned char sb[WR_CH * 64 / 256];
+    const bool sums = tk == 0 && !again;
+    if (t0 || again) ea_raw_barrier();     // the chunk (pass) before this one has been read
+    int sb[WR_CH * 64 / 256];
+    if (!end) {
+      const int left = (int)(m_end - mc);
+      const uint8_t* const sx = p.sx + tk * p.Rp + mc;
 #pragma unroll
-    for (int u = 0; u < WR_CH * 64 / 256; ++u) sb[u] = u * 256 + tid < left ? sx[u * 256 + tid] : 0;      // (a row that is not there: factor 0)
-    rd = ea_make_rows(p.dy + mc * p.N + n0, ((m_end - mc) * p.N - n0) * 2);
-    rx = ea_make_rows(p.x + mc * p.Kp + k0, (m_end - mc) * p.Kp - k0);
+      for (int u = 0; u < WR_CH * 64 / 256; ++u) sb[u] = sx[u * 256 + tid < left ? u * 256 + tid : left - 1];      // (behind the end: zeros, any factor)
+      rd = ea_make_rows(p.dy + mc * p.N + n0, ((m_end - mc) * p.N - n0) * 2);
+      rx = ea_make_rows(p.x + mc * p.Kp + k0, (m_end - mc) * p.Kp - k0);
 #pragma unroll
-    for (int t = 0; t < WR_S - 1; ++t)
-      if (t < n) stage(t);
+      for (int t = 0; t < WR_S - 1; ++t)
+        if (t < n) stage(t);
+      if (!again) {
+        unsigned w = 0;
 #pragma unroll
-    for (int u = 0; u < WR_CH * 64 / 256; ++u) *reinterpret_cast<f16*>(scl + (u * 256 + tid) * 2) = wl_factor(sb[u]);
+        for (int u = 0; u < WR_CH * 64 / 256; ++u) w = wx_max(w, wx_word(sb[u]));
+        wx_range_put(red, w);
+        ea_raw_barrier();
+        wx_range_get<0, 1, 4>(red, unit);
+      }
+    }
+    int from, to, old;
+    const bool away = unit.next(from, to, old);
+    if (end || away) put(old);
+    if (end) break;
+    wx_rescale(acc, away, old - unit.u);
+#pragma unroll
+    for (int u = 0; u < WR_CH * 64 / 256; ++u) *reinterpret_cast<f16*>(scl + (u * 256 + tid) * 2) = wl_factor(sb[u], unit.u, from, to);
     for (int t = 0; t < n; ++t) {
       if (t + WR_S - 2 < n) ea_wait_dma<(WR_S - 2) * 6>();           // (step t + WR_S - 2 has been issued: it alone may be in flight)
       else ea_wait_dma<0>();
@@ -384,17 +533,16 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
         }
       }
     }
+    again = unit.lo <= unit.hi;
+    if (!again) t0 += WR_CH;
   }
-  float* dw = p.dw + (long long)blockIdx.y * p.part;
   float* db = p.splits > 1 ? dw + (long long)p.N * p.K : p.db;
+  if (tk == 0 && lq == 0)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {            // D^T: a lane holds 4 consecutive k of one n
-    const int n = n0 + wm * 64 + (i ^ (2 * wn)) * 16 + l15;
-    if (n >= p.N) continue;
-    if (i < 2 && sums && lq == 0) db[n] = accb[i & 1][0];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wn * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
-  }
+    for (int i = 0; i < 2; ++i) {
+      const int n = n0 + wm * 64 + (i ^ (2 * wn)) * 16 + l15;
+      if (n < p.N) db[n] = accb[i][0];
+    }
 }
 
 __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams p) {
@@ -504,6 +652,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
 #endif
   };
   // dy's column sums, one accumulator's worth per workgroup: quadrants 0 by the first k tile, 1 by the second (there are two: wgrad_plan)
+  bool again = false;                      // another pass over the same chunk
   auto body = [&](int t, auto more_c) {
     constexpr bool more = decltype(more_c)::value;
     const char* buf = smem + (t & 1) * WL_STEP;
@@ -511,7 +660,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
     read_d(buf, c0);
     if (more) ea_wait_dma<2>(); else ea_wait_dma<0>();
     ea_f8l_barrier();
-    mma(c0, c0, fb0, tk == 0);
+    mma(c0, c0, fb0, tk == 0 && !again);
     ea_f8l_barrier();
     if (more) stage_d(0);
     read_x(t, c1, fb1);
@@ -523,7 +672,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
     read_d(buf, c1);
     if (more) ea_wait_dma<4>();
     ea_f8l_barrier();
-    mma(c1, c1, fb1, tk == 1);
+    mma(c1, c1, fb1, tk == 1 && !again);
     ea_f8l_barrier();
     if (more) {
       read_x(t + 1, c0, fbn);
@@ -538,26 +687,55 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
         for (int ks = 0; ks < 2; ++ks) fb0[j][ks] = fbn[j][ks];
     ea_f8l_barrier();
   };
-  for (; t0 < steps; t0 += WL_CH) {
+  unsigned* const red = reinterpret_cast<unsigned*>(smem + WL_RED);
+  WxUnit unit0, unit1;                     // of the tile's two block columns
+  float* const dw = p.dw + (long long)blockIdx.y * p.part;
+  const ea_rows out = ea_make_rows(dw + (long long)n0 * p.K, (long long)(p.N - n0) * p.K * 4);
+  bool stored = false;
+  auto put = [&](int u) {
+    wg_put(out, acc, [&](int i) { return wm * 128 + (i >> 2) * 64 + ((i & 3) ^ wn) * 16; }, l15, k0 + wn * 64 + 4 * lq, p.K, u, stored);
+    stored = true;
+  };
+  for (;;) {
+    const bool end = t0 >= steps;
     const int n = steps - t0 < WL_CH ? steps - t0 : WL_CH;
     const long long mc = m_begin + t0 * 64ll;
-    if (t0) ea_raw_barrier();              // the chunk before this one has been read
-    unsigned char sb[WL_CH * 128 / 512];
-    int kb = 2 * tk + ((tid >> 6) & 1);
-    if (kb >= (p.Kp >> 7)) kb = (p.Kp >> 7) - 1;
-    const int mt = (tid >> 7) * 64 + (tid & 63), left = (int)(m_end - mc);
-    const uint8_t* const sx = p.sx + kb * p.Rp + mc + mt;
+    if (t0 || again) ea_raw_barrier();     // the chunk (pass) before this one has been read
+    int sb[WL_CH * 128 / 512];
+    if (!end) {
+      int kb = 2 * tk + ((tid >> 6) & 1);
+      if (kb >= (p.Kp >> 7)) kb = (p.Kp >> 7) - 1;
+      const int mt = (tid >> 7) * 64 + (tid & 63), left = (int)(m_end - mc);
+      const uint8_t* const sx = p.sx + kb * p.Rp + mc;
 #pragma unroll
-    for (int u = 0; u < WL_CH * 128 / 512; ++u) sb[u] = mt + u * 256 < left ? sx[u * 256] : 0;      // (a row that is not there: factor 0)
-    rd = ea_make_rows(p.dy + mc * p.N + n0, ((m_end - mc) * p.N - n0) * 2);
-    rx = ea_make_rows(p.x + mc * p.Kp + k0, (m_end - mc) * p.Kp - k0);
-    begin(0);
-    stage_x(0);
-    stage_x(1);
-    stage_d(0);
-    stage_d(1);
+      for (int u = 0; u < WL_CH * 128 / 512; ++u) sb[u] = sx[mt + u * 256 < left ? mt + u * 256 : left - 1];      // (behind the end: zeros, any factor)
+      rd = ea_make_rows(p.dy + mc * p.N + n0, ((m_end - mc) * p.N - n0) * 2);
+      rx = ea_make_rows(p.x + mc * p.Kp + k0, (m_end - mc) * p.Kp - k0);
+      begin(0);
+      stage_x(0);
+      stage_x(1);
+      stage_d(0);
+      stage_d(1);
+      if (!again) {
+        unsigned w = 0;
 #pragma unroll
-    for (int u = 0; u < WL_CH * 128 / 512; ++u) *reinterpret_cast<f16*>(scl + (u * 512 + tid) * 2) = wl_factor(sb[u]);
+        for (int u = 0; u < WL_CH * 128 / 512; ++u) w = wx_max(w, wx_word(sb[u]));
+        wx_range_put(red, w);                // (even waves: the first block column, odd ones the second)
+        ea_raw_barrier();
+        wx_range_get<0, 2, 8>(red, unit0);
+        wx_range_get<1, 2, 8>(red, unit1);
+      }
+    }
+    int from0, to0, from1, to1, old0, old1;
+    const bool away0 = unit0.next(from0, to0, old0), away1 = unit1.next(from1, to1, old1);
+    const bool away = wn >> 1 ? away1 : away0;
+    const int old = wn >> 1 ? old1 : old0;
+    if (end || away) put(old);
+    if (end) break;
+    wx_rescale(acc, away, old - (wn >> 1 ? unit1.u : unit0.u));
+    const int fu = wave & 1 ? unit1.u : unit0.u, from = wave & 1 ? from1 : from0, to = wave & 1 ? to1 : to0;
+#pragma unroll
+    for (int u = 0; u < WL_CH * 128 / 512; ++u) *reinterpret_cast<f16*>(scl + (u * 512 + tid) * 2) = wl_factor(sb[u], fu, from, to);
     ea_wait_dma<2>();
     ea_raw_barrier();
     read_x(0, c0, fb0);
@@ -565,16 +743,10 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
     for (int t = 0; t + 1 < n; ++t) body(t, std::true_type{});
     body(n - 1, std::false_type{});
     if (wm == 0) ea_f8l_barrier();         // both wave rows execute the same number of barriers
+    again = unit0.lo <= unit0.hi || unit1.lo <= unit1.hi;
+    if (!again) t0 += WL_CH;
   }
-  float* dw = p.dw + (long long)blockIdx.y * p.part;
   float* db = p.splits > 1 ? dw + (long long)p.N * p.K : p.db;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {            // D^T: a lane holds 4 consecutive k of one n
-    const int n = n0 + wm * 128 + (i >> 2) * 64 + ((i & 3) ^ wn) * 16 + l15;
-    if (n >= p.N) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) wg_store4(dw + (long long)n * p.K, k0 + wn * 64 + j * 16 + 4 * lq, p.K, acc[i][j]);
-  }
   if (tk < 2 && lq == 0) {
     const int n = n0 + wm * 128 + tk * 64 + wn * 16 + l15;
     if (n < p.N) db[n] = accb[0];
@@ -604,6 +776,7 @@ struct WgradPlan { int kernel, splits, rows; };
 WgradPlan wgrad_plan(int M, int N, int K) {
   WgradPlan w{-1, 1, 64};
   const int v = ea_forced_variant();       // tests: 101, 102, 103 pin a kernel
+  const int f = ea_forced_splits() < (M + 63) / 64 ? ea_forced_splits() : 0;
   const bool large = K > 256;              // (two k tiles: each sums one half of its dy columns for db)
   const bool dma = (N & 7) == 0 && N <= (1 << 18) && K <= (1 << 18) && v != 103;
   const double nk = (double)N * K;
@@ -616,6 +789,7 @@ WgradPlan wgrad_plan(int M, int N, int K) {
     for (int s = 1; s <= steps && s <= 64; ++s) {
       const int per = (steps + s - 1) / s;
       if ((steps + per - 1) / per != s) continue;                    // (this many slices leave one empty)
+      if (f && s != f) continue;
       const long long wgs = tiles * s;
       const double t = (kernel == 256 ? (wgs + 255) / 256 * (per * 1.65 + 10)
                                       : wgs / 512 * (per * 1.25 + 5) + (wgs % 512 > 256 ? per * 1.25 + 5 : wgs % 512 ? per * 0.87 + 5 : 0)) +
@@ -731,7 +905,7 @@ extern "C" int ea_gemm_fp8_wgrad(const void* dy, const void* x, const unsigned c
     EA_LAUNCH(k, dim3((unsigned)tiles, p.splits), dim3(256), WR_LDS, stream, p);
   } else {
     auto k = ea_fp8_wgrad_kernel;
-    EA_LAUNCH(k, dim3((unsigned)tiles, p.splits), dim3(256), 2 * WG_BUF, stream, p);
+    EA_LAUNCH(k, dim3((unsigned)tiles, p.splits), dim3(256), WG_LDS, stream, p);
   }
   int st = ea_launch_status();
   if (st != EA_OK || p.splits == 1) return st;

@@ -841,6 +841,7 @@ static int launch_pair(EaGemmParams& p, EaGemmParams& q, void* workspace, size_t
 }  // namespace
 
 int ea_forced_variant() { return g_tune.variant; }
+int ea_forced_splits() { return g_tune.splits; }
 
 extern "C" int ea_set_tuning(const ea_tuning* t) {
   if (t) g_tune = *t;

@@ -1281,8 +1281,8 @@ def gemm_fp8(a, w, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=t
 
 
 def gemm_fp8_wgrad(dy, x):
-    """Gradients of a Linear's weight and bias from its 8-bit input: dy fp16 [..., N], x an Fp8Tensor of rows [..., K] (|values| <=
-    114688) -> (dw fp32 [N, K] = dy^T x, db fp32 [N]), both summed in fp32 in a fixed order."""
+    """Gradients of a Linear's weight and bias from its 8-bit input: dy fp16 [..., N], x an Fp8Tensor of rows [..., K], of any size that the
+    format holds -> (dw fp32 [N, K] = dy^T x, db fp32 [N]), both summed in fp32 in a fixed order; every product is exact."""
     M, N = _lead(dy, (_F16,))
     if not (N and M <= _MOST_ROWS and _is_rows(x) and x.rows == M):
         _refuse("gemm_fp8_wgrad: dy must be fp16 [..., N] of at most 2^30 rows, x an Fp8Tensor of as many rows", dy=dy, x=x)

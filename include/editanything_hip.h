@@ -434,7 +434,8 @@ int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const unsigned c
 int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K,
                 const ea_epilogue* e, void* stream);
 /* Gradients of a Linear's weight and bias from its 8-bit input: dw fp32 [N][K] = dy^T x, db fp32 [N] = column sums of dy (fp16 [M][N]).
- * A block of x whose maximum exceeds 114688 decodes to infinities.  The sums have a fixed order. */
+ * x may hold any exponents; its products with dy are exact.  Rows further apart than 2^22 within 2048 rows of a block column are taken in several passes
+ * (an infinity of dy then gives NaN).  The sums have a fixed order. */
 size_t ea_gemm_fp8_wgrad_workspace_bytes(int M, int N, int K);
 int ea_gemm_fp8_wgrad(const void* dy, const void* x, const unsigned char* x_scale, float* dw, float* db, int M, int N, int K, void* workspace,
                       size_t ws_bytes, void* stream);

@@ -112,6 +112,7 @@ SIGNATURES = {
     "ea_layernorm_bwd_workspace_bytes": (_sz, [_i, _i]),
     "ea_layernorm_bwd": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp]),
     "ea_gemm_fp8": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, C.POINTER(Epilogue), _vp]),
+    "ea_gemm_fp8_exact": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, C.POINTER(Epilogue), _vp]),
     "ea_gemm_fp8_wgrad_workspace_bytes": (_sz, [_i, _i, _i]),
     "ea_gemm_fp8_wgrad": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
     "ea_gather_rows": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp]),

@@ -383,16 +383,13 @@ __device__ __forceinline__ void wl_dma16(ea_rows r, unsigned off, char* lds_base
 }
 // 8 codes times their rows' factors
 __device__ __forceinline__ f16x8 wl_decode8(u32x2 w, f16x8 s) {
+  const f16x8 h = ea_f8_half8(w[0], w[1], 0.00390625f);
 #ifdef EA_EMU
   f16x8 o;
-  for (int j = 0; j < 8; ++j) o[j] = (f16)((float)(f16)(ea_emu_fp8_to_f32((w[j >> 2] >> (8 * (j & 3))) & 255) * 0.00390625f) * (float)s[j]);
+  for (int j = 0; j < 8; ++j) o[j] = (f16)((float)h[j] * (float)s[j]);
   return o;
 #else
-  const u32x4 h = {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 0.00390625f, false)),
-                   __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 0.00390625f, true)),
-                   __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], 0.00390625f, false)),
-                   __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[1], 0.00390625f, true))};
-  return __builtin_bit_cast(f16x8, h) * s;
+  return h * s;
 #endif
 }
 // 2^(E - U + 8) as fp16 from the stored byte (-7 ... 15 inside a window; less where the unit could not follow); 0 for a row of another pass
@@ -805,9 +802,9 @@ WgradPlan wgrad_plan(int M, int N, int K) {
 
 long long fp8_tiles(const EaFp8GemmParams& p, int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); }
 
-template <int BM, int BN, int WM, int WN, int S>
+template <int BM, int BN, int WM, int WN, int S, bool EXACT = false>
 int fp8_ring_launch(const EaFp8GemmParams& p, void* stream) {
-  auto k = ea_fp8_ring_kernel<BM, BN, WM, WN, S>;
+  auto k = ea_fp8_ring_kernel<BM, BN, WM, WN, S, EXACT>;
   const int smem = (BM + BN) * 128 * S + EA_F8_CH * (BM + 4);
   const long long tiles = fp8_tiles(p, BM, BN);
   if (tiles > 0x7fffffffll) return EA_ERR_BAD_SHAPE;
@@ -842,11 +839,20 @@ int fp8_launch(EaFp8GemmParams& p, void* stream) {
   if (v == 103 || (v < 101 && fp8_tiles(p, 64, 128) >= 160)) return fp8_ring_launch<64, 128, 2, 4, 2>(p, stream);
   return fp8_ring_launch<64, 64, 2, 2, 4>(p, stream);
 }
+// The same with exact products (the 8-bit kernels' time behind it): 128 x 128 from 512 tiles on: 16384 x 5120 x 1280 252 us (64 x 128: 292, 64 x 64:
+// 369; 111), 32768 x 320 x 320 18.2 (19.9, 23.9; 12.1), 8192^3 1029 = 1070 TFLOP/s (390); but 8192 x 640 x 640, 320 tiles, 17.0 (15.4, 18.0; 10.2).
+// 64 x 128 from 160 tiles on: 616 x 2560 x 1024 9.7 (64 x 64: 10.6; 6.6), 2048 x 1280 x 1280 16.5 (17.8; 9.6).  64 x 64 below: 512 x 1280 x
+// 5120 25.5 (64 x 128: 31.5; 15.0).
+int fp8_exact_launch(EaFp8GemmParams& p, void* stream) {
+  p.raster_gm = 8;
+  const int v = ea_forced_variant();
+  if (v == 102 || (v < 101 && fp8_tiles(p, 128, 128) >= 512)) return fp8_ring_launch<128, 128, 2, 2, 2, true>(p, stream);
+  if (v == 103 || (v < 101 && fp8_tiles(p, 64, 128) >= 160)) return fp8_ring_launch<64, 128, 2, 4, 2, true>(p, stream);
+  return fp8_ring_launch<64, 64, 2, 2, 4, true>(p, stream);
+}
 
-}  // namespace
-
-extern "C" int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K,
-                           const ea_epilogue* e, void* stream) {
+int gemm_fp8_entry(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K, const ea_epilogue* e,
+                   bool exact, void* stream) {
   if (!a || !a_scale || !w || !w_scale || !e || !e->out) return EA_ERR_BAD_ARG;
   if (M <= 0 || N <= 0 || K <= 0 || M > EA_FP8_ROWS || N > (1 << 22) || K > (1 << 20)) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)a & 15) || ((uintptr_t)w & 15) || ((uintptr_t)a_scale & 3)) return EA_ERR_BAD_ARG;
@@ -864,7 +870,18 @@ extern "C" int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const vo
   p.vec = (N & 7) == 0 && (e->ldc & 7) == 0 && e->ldc < (1 << 21) && ((uintptr_t)e->out & 15) == 0;
   if (e->residual || e->residual32)
     p.vec = p.vec && (e->ldr & 7) == 0 && e->ldr < (1 << 21) && ((((uintptr_t)e->residual) | ((uintptr_t)e->residual32)) & 15) == 0;
-  return fp8_launch(p, stream);
+  return exact ? fp8_exact_launch(p, stream) : fp8_launch(p, stream);
+}
+
+}  // namespace
+
+extern "C" int ea_gemm_fp8(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K,
+                           const ea_epilogue* e, void* stream) {
+  return gemm_fp8_entry(a, a_scale, w, w_scale, M, N, K, e, false, stream);
+}
+extern "C" int ea_gemm_fp8_exact(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K,
+                                 const ea_epilogue* e, void* stream) {
+  return gemm_fp8_entry(a, a_scale, w, w_scale, M, N, K, e, true, stream);
 }
 
 extern "C" size_t ea_gemm_fp8_wgrad_workspace_bytes(int M, int N, int K) {

@@ -119,3 +119,93 @@ def test_wgrad_units_change_along_a_slice(kb, kernel):
     # either sign -- together far below 32 u32 of the sum of magnitudes (n s)
     assert (np.abs(dw - d.T @ x) <= 32 * U32 * (np.abs(d).T @ np.abs(x)) + FLUSH).all()
     assert (np.abs(db - d.sum(0)) <= 32 * U32 * np.abs(d).sum(0)).all()
+
+
+# ---------------------------------------------------------------------------------------------- products with fp32 accuracy
+@pytest.mark.parametrize("kernel", [0, 102, 103, 104])
+@pytest.mark.parametrize("form", ["plain", "bias gelu fp32", "bias silu residual", "residual32 scale"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (16, 8, 130), (70, 100, 300), (130, 136, 640), (33, 7, 77)])
+def test_gemm_fp8_exact(kb, M, N, K, form, kernel):
+    """The bound of test_gemm_fp8 without the matrix unit's share: only fp32 roundings are left."""
+    force(kb, kernel)
+    aq, sa, wq, sw, ref, mag = gemm_case(M, N, K, 41)
+    g = np.random.default_rng(42)
+    f32out = "fp32" in form
+    out = kb.up(np.full((M + 1, N), 7, np.float32 if f32out else np.float16))
+    bias = g.standard_normal(N).astype(np.float32) if "bias" in form else None
+    res = g.standard_normal((M, N)).astype(np.float16) if "residual" in form and "32" not in form else None
+    res32 = g.standard_normal((M, N)).astype(np.float32) if "residual32" in form else None
+    act = GELU if "gelu" in form else SILU if "silu" in form else 0
+    scale = 0.5 if "scale" in form else 1.0
+    e = epilogue(out, bias=bias, act=act, scale=scale, residual=res, residual32=res32)
+    assert kb.lib.ea_gemm_fp8_exact(ptr(aq), ptr(sa), ptr(wq), ptr(sw), M, N, K, ctypes.byref(e), kb.stream) == 0
+    v = ref + (0 if bias is None else bias.astype(np.float64))
+    err = 2 * (K + 2) * U32 * mag + U32 * np.abs(v)
+    if act:
+        err = 1.13 * err + ACT_ABS + 4 * U32 * np.abs(v)           # (neither slope exceeds 1.13)
+        v = act64(v, act)[0]
+    v = scale * v + (0 if res is None else res.astype(np.float64)) + (0 if res32 is None else res32.astype(np.float64))
+    got = kb.down(out)
+    assert (got[M] == 7).all()
+    assert (np.abs(got[:M] - v) <= scale * err + (2 * U32 if f32out else U16) * np.abs(v) + TINY16 + 4 * U32 * np.abs(v)).all()
+
+
+@pytest.mark.parametrize("signs", ["random", "alternating"])
+@pytest.mark.parametrize("kernel", [0, 102, 103, 104])
+def test_gemm_fp8_exact_small_products_beside_a_large_one(kb, kernel, signs):
+    """One product of 2^16 and seven of 2^-2 in each eight neighbours: the 8-bit instruction cuts the seven away, this one may not.  K runs over
+    two chunks of scale bytes; a NaN code reaches its row only; the exponents lie far apart."""
+    M, N, K = 20, 24, 8450
+    nb = -(-K // 128)
+    a, w = np.zeros((M, nb * 128)), np.zeros((N, nb * 128))
+    a[:, :K], w[:, :K] = 0.5, 0.5
+    a[:, 3:K:8], w[:, 3:K:8] = 256, 256
+    g = np.random.default_rng(43)
+    if signs == "random":
+        a[:, :K] *= np.where(g.random((M, K)) < 0.5, 1, -1)
+    else:
+        a[:, 3:K:16] = -256                                    # the large ones cancel, the small ones add up
+    ea, ew = np.zeros((nb, M), np.int64), np.zeros((nb, 1), np.int64)
+    ea[1::2], ew[1::2] = 100, -100                             # the product's exponent is 0, its factors' are not
+    aq, wq = encode(a), encode(w)
+    aq[4, 200] = 0x7F
+    out = kb.up(np.full((M + 1, N), 7, np.float32))
+    force(kb, kernel)
+    assert kb.lib.ea_gemm_fp8_exact(ptr(aq), ptr(pack_scales(ea)), ptr(wq), ptr((ew + 127).astype(np.uint8)), M, N, K, ctypes.byref(epilogue(out)),
+                                    kb.stream) == 0
+    got = kb.down(out)
+    assert (got[M] == 7).all() and np.isnan(got[4]).all()
+    keep = np.arange(M) != 4
+    # A block's sum is a multiple of 2^-2 below 2^21: exact.  Behind a block the accumulator is below `top`; below 2^22 it is exact too, below 2^23 the
+    # addition of a block rounds to multiples of 2^-1, off by 2^-2 at most, once for each of the 67 blocks
+    top = np.abs(np.cumsum([a[:, b * 128:b * 128 + 128] @ w[:, b * 128:b * 128 + 128].T for b in range(nb)], 0)).max()
+    assert top < 2 ** 23
+    assert (np.abs(got[:M] - a @ w.T)[keep] <= (0 if top < 2 ** 22 else nb * 0.25)).all()
+    if signs == "alternating":
+        assert top < 2 ** 22 and (np.abs(a @ w.T) > 1800).all()
+
+
+def test_gemm_fp8_exact_refuses_as_gemm_fp8(emu_lib):
+    a = np.zeros((256, 256), np.float32)
+    p = a.ctypes.data
+    e = epilogue(a)
+    f = lambda M=16, N=16, K=128, q=p: emu_lib.ea_gemm_fp8_exact(q, p, p, p, M, N, K, ctypes.byref(e), None)  # noqa: E731
+    assert f(q=None) == -2 and f(q=p + 8) == -2 and f(M=0) == f(N=-1) == f(K=1 << 21) == f(M=(1 << 30) + 1) == -1 and f(N=512) == -2
+    e.act = GEGLU
+    assert f() == -3
+
+
+@pytest.mark.gpu
+def test_an_fp32_product_is_exact_unless_told_otherwise():
+    g = torch.Generator(device="cuda").manual_seed(44)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    for M, N, K in ((616, 2560, 1024), (8192, 640, 640), (33, 24, 320), (8192, 1280, 320)):
+        a, w = ops.quantize_fp8(r(M, K)), ops.quantize_fp8_weight(r(N, K) * K ** -0.5)
+        x, y = a.dequantize(torch.float32).double(), w.dequantize(torch.float32).double().t().contiguous()
+        ref, mag = x @ y, x.abs() @ y.abs()
+        got = {k: ops.gemm_fp8(a, w, out_dtype=torch.float32, exact=k).double() for k in (None, True, False)}
+        assert torch.equal(got[None], got[True])
+        assert ((got[True] - ref).abs() <= 2 * (K + 2) * U32 * mag + 4 * U32 * ref.abs()).all()
+        assert ((got[False] - ref).abs() <= (2 * (K + 2) * U32 + UNIT) * mag + 4 * U32 * ref.abs()).all()
+        half = {k: ops.gemm_fp8(a, w, exact=k) for k in (None, True, False)}
+        assert torch.equal(half[None], half[False]) and torch.equal(half[True], got[True].to(torch.float32).half())

@@ -213,11 +213,9 @@ __device__ __forceinline__ u32x2 ea_fp8_block(const V& v, int& byte) {
   return u32x2{ea_fp8_pack4(t[0], t[1], t[2], t[3]), ea_fp8_pack4(t[4], t[5], t[6], t[7])};
 }
 
-// GELU by the polynomial of ea_gelu_erf (ea_platform.h) and to its values.  That takes fmaxf(x, 0) and puts a NaN back afterwards; the
-// comparison x < 0 lets a NaN through by itself, one instruction less.  The epilogue of the 256 x 256 product is bound by these
-// instructions: with the scale's multiplication left out where it is 1, 16384 x 5120 x 1280 went from 137 to 128 us.
-__device__ __forceinline__ float ea_fp8_gelu(float x) {
-  const float a = fminf(fabsf(x), 5.65685424949238f);
+// 1 - Phi(a) = erfc(a / sqrt 2) / 2 by the polynomial of ea_gelu_erf (ea_platform.h), for a = |x| up to 4 sqrt 2
+#define EA_FP8_GELU_END 5.65685424949238f
+__device__ __forceinline__ float ea_fp8_gelu_tail(float a) {
   float q = -4.276626896171365e-06f;
   q = q * a + 1.2775987670465838e-05f;
   q = q * a + 0.0005758762708865106f;
@@ -225,7 +223,14 @@ __device__ __forceinline__ float ea_fp8_gelu(float x) {
   q = q * a + 0.05294874310493469f;
   q = q * a + 0.45904383063316345f;
   q = q * a + 1.1511269807815552f;
-  return (x < 0.0f ? 0.0f : x) - a * ea_exp2_raw(-a * q - 1.0f);
+  return ea_exp2_raw(-a * q - 1.0f);
+}
+// GELU to ea_gelu_erf's values.  That takes fmaxf(x, 0) and puts a NaN back afterwards; the
+// comparison x < 0 lets a NaN through by itself, one instruction less.  The epilogue of the 256 x 256 product is bound by these
+// instructions: with the scale's multiplication left out where it is 1, 16384 x 5120 x 1280 went from 137 to 128 us.
+__device__ __forceinline__ float ea_fp8_gelu(float x) {
+  const float a = fminf(fabsf(x), EA_FP8_GELU_END);
+  return (x < 0.0f ? 0.0f : x) - a * ea_fp8_gelu_tail(a);
 }
 
 #define EA_FP8_ROWS (1 << 30)      // most rows of an entry that counts them in 32 bits: tile counts and row indexes stay below 2^31

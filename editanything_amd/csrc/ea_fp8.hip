@@ -222,17 +222,10 @@ struct ActParams {
 template <int ACT>
 __device__ __forceinline__ float act_f(float z) { return ACT == EA_ACT_SILU ? ea_silu(z) : ea_fp8_gelu(z); }
 
-// Phi(x) and x phi(x); 1 - Phi(a) = erfc(a / sqrt 2) / 2 as in ea_gelu_erf
-__device__ __forceinline__ void gelu_parts(float x, float& phi_c, float& xp) {
-  const float a = fminf(fabsf(x), 5.65685424949238f);
-  float q = -4.276626896171365e-06f;
-  q = q * a + 1.2775987670465838e-05f;
-  q = q * a + 0.0005758762708865106f;
-  q = q * a - 0.007670961786061525f;
-  q = q * a + 0.05294874310493469f;
-  q = q * a + 0.45904383063316345f;
-  q = q * a + 1.1511269807815552f;
-  const float t = ea_exp2_raw(-a * q - 1.0f);
+// GELU(x) as in the forward pass, Phi(x) and x phi(x).  (x Phi(x) would not do for GELU(x): Phi ends at 7.7e-9, not at 0, and x does not end)
+__device__ __forceinline__ void gelu_parts(float x, float& gelu, float& phi_c, float& xp) {
+  const float a = fminf(fabsf(x), EA_FP8_GELU_END), t = ea_fp8_gelu_tail(a);
+  gelu = (x < 0.0f ? 0.0f : x) - a * t;
   phi_c = x > 0.0f ? 1.0f - t : t;
   xp = x * 0.3989422804014327f * ea_exp2_raw(fmaxf(x * x * -0.7213475204444817f, -126.0f));
   if (x != x) phi_c = xp = x;
@@ -243,8 +236,8 @@ __device__ __forceinline__ float act_slope(float z) {
     const float s = 1.0f / (1.0f + ea_expf(-z));
     return s * (1.0f + z * (1.0f - s));
   }
-  float P, xp;
-  gelu_parts(z, P, xp);
+  float f, P, xp;
+  gelu_parts(z, f, P, xp);
   return P + xp;
 }
 
@@ -297,9 +290,9 @@ __global__ __launch_bounds__(256) void ea_act_use_kernel(ActParams p) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if constexpr (G == 2) {
-        float P, xp;
-        gelu_parts(z[1][j], P, xp);
-        o[0][j] = d[j] * (z[1][j] * P);
+        float f, P, xp;
+        gelu_parts(z[1][j], f, P, xp);
+        o[0][j] = d[j] * f;
         o[1][j] = d[j] * z[0][j] * (P + xp);
       } else o[0][j] = d[j] * act_slope<ACT>(z[0][j]);
     }

@@ -209,3 +209,28 @@ def test_an_fp32_product_is_exact_unless_told_otherwise():
         assert ((got[False] - ref).abs() <= (2 * (K + 2) * U32 + UNIT) * mag + 4 * U32 * ref.abs()).all()
         half = {k: ops.gemm_fp8(a, w, exact=k) for k in (None, True, False)}
         assert torch.equal(half[None], half[False]) and torch.equal(half[True], got[True].to(torch.float32).half())
+
+
+# -------------------------------------------------------------------------------------------------------- activations, backward
+@pytest.mark.parametrize("H", [128, 77])
+def test_geglu_value_gradient_of_strongly_negative_gates(kb, H):
+    """dvalue = dh gelu(gate): it vanishes with the gate's GELU, however large the gate is."""
+    gates = -np.array([0.5, 3, 5.5, 5.7, 8, 30, 100, 1000, 8192, 28672, 57344])
+    z = np.zeros((2 * len(gates), H), np.float32)
+    z[0::2], z[1::2] = 3.0, gates[:, None]
+    z[1::2, 1::2] *= -1                                        # and positive ones, where it is the gate
+    q, e = quantize(z)
+    M, v = len(gates), values(q, e, H)
+    dh = np.full((M, H), 100, np.float16)
+    dh[:, 2] = -100
+    dz = kb.zeros((M, 2 * H), np.float16)
+    assert kb.lib.ea_activation_fp8_bwd(ptr(dh), ptr(q), ptr(pack_scales(e)), GEGLU, ptr(dz), M, H, kb.stream) == 0
+    with np.errstate(over="ignore"):
+        ref = dh.astype(np.float64) * act64(v[1::2], GELU)[0]
+        want = np.where(np.abs(ref) >= 65520, np.copysign(np.inf, ref), ref)
+    got = kb.down(dz)[:, :H].astype(np.float64)
+    inf = np.isinf(want)
+    assert (got[inf] == want[inf]).all()
+    # the GELU is off by ACT_ABS at most, wherever the gate lies
+    got, ref = np.where(inf, 0, got), np.where(inf, 0, ref)
+    assert (np.abs(got - ref) <= U16 * np.abs(ref) + TINY16 + ACT_ABS * 100 + 8 * U32 * np.abs(ref)).all()

@@ -227,14 +227,15 @@ __device__ __forceinline__ void gelu_parts(float x, float& gelu, float& phi_c, f
   const float a = fminf(fabsf(x), EA_FP8_GELU_END), t = ea_fp8_gelu_tail(a);
   gelu = (x < 0.0f ? 0.0f : x) - a * t;
   phi_c = x > 0.0f ? 1.0f - t : t;
-  xp = x * 0.3989422804014327f * ea_exp2_raw(fmaxf(x * x * -0.7213475204444817f, -126.0f));
+  const float c = fminf(fmaxf(x, -13.0f), 13.0f);              // (phi(13) = 8e-38: the exponent ends inside fp32's, and so does x)
+  xp = c * 0.3989422804014327f * ea_exp2_raw(c * c * -0.7213475204444817f);
   if (x != x) phi_c = xp = x;
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if (ACT == EA_ACT_SILU) {
-    const float s = 1.0f / (1.0f + ea_expf(-z));
-    return s * (1.0f + z * (1.0f - s));
+    const float s = 1.0f / (1.0f + ea_expf(-z)), c = fminf(fmaxf(z, -200.0f), 200.0f);      // (1 - s or s is 0 there; a NaN is in s)
+    return s * (1.0f + c * (1.0f - s));
   }
   float f, P, xp;
   gelu_parts(z, f, P, xp);

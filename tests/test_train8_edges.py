@@ -234,3 +234,26 @@ def test_geglu_value_gradient_of_strongly_negative_gates(kb, H):
     # the GELU is off by ACT_ABS at most, wherever the gate lies
     got, ref = np.where(inf, 0, got), np.where(inf, 0, ref)
     assert (np.abs(got - ref) <= U16 * np.abs(ref) + TINY16 + ACT_ABS * 100 + 8 * U32 * np.abs(ref)).all()
+
+
+@pytest.mark.parametrize("act", [SILU, GELU, GEGLU])
+def test_slopes_of_the_largest_inputs(kb, act):
+    """Inputs that only an Fp8Tensor of an fp32 tensor holds, up to what decodes to infinity: the slope is 0 or 1, a GEGLU's value gradient the
+    gate or 0."""
+    g = 2 if act == GEGLU else 1
+    x = np.zeros((16, 128), np.float32)
+    x[:, 0::2] = np.array([20, 100, 1e3, 7e4, 1e6, 3e10, 1e18, 1e19, 3e20, 1e30, 3e36, 1e37, 1e38, 2e38, 3e38, np.finfo(np.float32).max])[:, None]
+    x[:, 1::2] = -x[:, 0::2]
+    z = np.ones((16 * g, 128), np.float32)
+    z[g - 1::g] = x
+    q, e = quantize(z)
+    dh = np.full((16, 128), 2, np.float16)
+    dz = kb.zeros((16, g * 128), np.float16)
+    assert kb.lib.ea_activation_fp8_bwd(ptr(dh), ptr(q), ptr(pack_scales(e)), act, ptr(dz), 16, 128, kb.stream) == 0
+    got = kb.down(dz).astype(np.float64)
+    want = np.where(x > 0, 2.0, 0.0)
+    assert (np.abs(got[:, -128:] - want) <= U16 * want + ACT_ABS * 2 + TINY16).all()
+    if g == 2:                             # the value's gradient: 2 gate or 0, infinite from 65520 on
+        v = 2 * np.where(x > 0, values(q, e, 128)[1::2], 0.0)
+        big = v >= 65520
+        assert np.isposinf(got[:, :128][big]).all() and (np.abs(got[:, :128] - v)[~big] <= U16 * v[~big] + 2 * ACT_ABS + TINY16).all()

@@ -234,5 +234,7 @@ __device__ __forceinline__ float ea_fp8_gelu(float x) {
 }
 
 #define EA_FP8_ROWS (1 << 30)      // most rows of an entry that counts them in 32 bits: tile counts and row indexes stay below 2^31
+// a launch holds fewer than 2^32 threads along x
+static inline bool ea_launch_holds(long long workgroups, int threads) { return workgroups * threads < (1ll << 32); }
 static inline int ea_fp8_blocks(int cols) { return (cols + EA_FP8_BLOCK - 1) / EA_FP8_BLOCK; }
 static inline long long ea_fp8_scale_pitch(long long rows) { return (rows + 15) / 16 * 16; }

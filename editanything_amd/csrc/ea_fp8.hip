@@ -305,11 +305,12 @@ __global__ __launch_bounds__(256) void ea_act_use_kernel(ActParams p) {
 bool al16(const void* a, const void* b = nullptr, const void* c = nullptr) {
   return ((((uintptr_t)a) | ((uintptr_t)b) | ((uintptr_t)c)) & 15) == 0;
 }
-// workgroups of 16 rows x Q_KB blocks, column tiles fastest; 0: more than a grid holds
+// workgroups of 16 rows x Q_KB blocks, column tiles fastest; 0: more than a launch holds
 unsigned q_grid(long long rows, int nb, int& gx) {
   gx = (nb + Q_KB - 1) / Q_KB;
+  if (rows > (1ll << 40)) return 0u;
   const long long g = (rows + 15) / 16 * gx;
-  return g > 0x7fffffffll ? 0u : (unsigned)g;
+  return ea_launch_holds(g, 256) ? (unsigned)g : 0u;
 }
 
 }  // namespace

@@ -807,14 +807,14 @@ int fp8_ring_launch(const EaFp8GemmParams& p, void* stream) {
   auto k = ea_fp8_ring_kernel<BM, BN, WM, WN, S, EXACT>;
   const int smem = (BM + BN) * 128 * S + EA_F8_CH * (BM + 4);
   const long long tiles = fp8_tiles(p, BM, BN);
-  if (tiles > 0x7fffffffll) return EA_ERR_BAD_SHAPE;
+  if (!ea_launch_holds(tiles, 64 * WM * WN)) return EA_ERR_BAD_SHAPE;
   ea_allow_big_lds(k, smem);
   EA_LAUNCH(k, dim3((unsigned)tiles), dim3(64 * WM * WN), smem, stream, p);
   return ea_launch_status();
 }
 int fp8_large_launch(const EaFp8GemmParams& p, void* stream) {
   const long long tiles = fp8_tiles(p, 256, 256);
-  if (tiles > 0x7fffffffll) return EA_ERR_BAD_SHAPE;
+  if (!ea_launch_holds(tiles, 512)) return EA_ERR_BAD_SHAPE;
   auto k = ea_fp8_large_kernel;
   ea_allow_big_lds(k, EA_F8L_LDS);
   EA_LAUNCH(k, dim3((unsigned)tiles), dim3(512), EA_F8L_LDS, stream, p);
@@ -911,7 +911,8 @@ extern "C" int ea_gemm_fp8_wgrad(const void* dy, const void* x, const unsigned c
   p.db = db;
   p.vec = (N & 7) == 0 && ((uintptr_t)dy & 15) == 0;
   const long long tiles = (long long)p.tiles_n * p.tiles_k;
-  if (tiles > 0x7fffffffll) return EA_ERR_BAD_SHAPE;
+  const long long total = (long long)N * K + N;
+  if (!ea_launch_holds(tiles, 512) || (p.splits > 1 && !ea_launch_holds((total + 255) / 256, 64))) return EA_ERR_BAD_SHAPE;
   if (kernel == 256) {
     auto k = ea_fp8_wgrad_large_kernel;
     ea_allow_big_lds(k, WL_LDS);
@@ -927,7 +928,6 @@ extern "C" int ea_gemm_fp8_wgrad(const void* dy, const void* x, const unsigned c
   int st = ea_launch_status();
   if (st != EA_OK || p.splits == 1) return st;
   auto j = ea_fp8_wgrad_join_kernel;
-  const long long total = (long long)N * K + N;
   EA_LAUNCH(j, dim3((unsigned)((total + 255) / 256)), dim3(64), 0, stream, (const float*)workspace, dw, db, (long long)N * K, total, p.splits);
   return ea_launch_status();
 }

@@ -445,6 +445,7 @@ int ln_lanes(int C) { return C <= 384 ? 16 : C <= 768 ? 32 : 64; }       // lane
 template <int XK, bool ANY, bool OUT8>
 int ln_train_launch(const LnTrainParams& p, void* stream) {
   const int lpr = ln_lanes(p.C), rows = 4 * (64 / lpr);
+  if (!ea_launch_holds((p.M + rows - 1) / rows, 256)) return EA_ERR_BAD_SHAPE;
   auto k = lpr == 16 ? ea_ln_train_kernel<XK, ANY, 16, 3, OUT8> : lpr == 32 ? ea_ln_train_kernel<XK, ANY, 32, 3, OUT8>
          : p.C <= 1536 ? ea_ln_train_kernel<XK, ANY, 64, 3, OUT8> : p.C <= 2560 ? ea_ln_train_kernel<XK, ANY, 64, 5, OUT8>
          : ea_ln_train_kernel<XK, ANY, 64, 8, OUT8>;
@@ -477,6 +478,7 @@ bool ln_bwd_few(int M) {
 template <int XK, bool F32, bool ANY>
 int ln_bwd_few_launch(const LnBwdParams& p, float* dgamma, float* dbeta, void* stream) {
   const int lpr = ln_lanes(p.C), rows = 4 * (64 / lpr), ncol = (p.C + LF_COLS - 1) / LF_COLS;
+  if (!ea_launch_holds(ncol + (long long)(p.M + rows - 1) / rows, 256)) return EA_ERR_BAD_SHAPE;
   auto k = lpr == 16 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 16, 3> : lpr == 32 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 32, 3>
          : p.C <= 1536 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 3> : p.C <= 2560 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 5>
          : ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 8>;

@@ -10,7 +10,7 @@ import torch
 from editanything_amd import _lib as L
 from editanything_amd import ops
 from emu_util import epilogue, ptr
-from test_train8 import (ACT_ABS, GEGLU, GELU, SILU, TINY16, U16, U32, UNIT, act64, decode, encode, force, gemm_case, pack_scales, quantize,
+from test_train8 import (ACT_ABS, GEGLU, GELU, KERNELS, SILU, TINY16, U16, U32, UNIT, act64, decode, encode, force, gemm_case, pack_scales, quantize,
                          quantize_weight, rows, values)
 
 FLUSH = 2.0 ** -126                        # fp32's smallest normal number: what lies below may be flushed
@@ -257,3 +257,31 @@ def test_slopes_of_the_largest_inputs(kb, act):
         v = 2 * np.where(x > 0, values(q, e, 128)[1::2], 0.0)
         big = v >= 65520
         assert np.isposinf(got[:, :128][big]).all() and (np.abs(got[:, :128] - v)[~big] <= U16 * v[~big] + 2 * ACT_ABS + TINY16).all()
+
+
+# ------------------------------------------------------------------------------------------------------------------ refusals
+def test_more_than_a_launch_holds_is_refused(emu_lib):
+    """2^32 threads along x are one too many; nothing is read or written before the refusal."""
+    lib = emu_lib
+    a = np.zeros((256, 256), np.float32)
+    p, o = a.ctypes.data, a.ctypes.data + 65536
+    for C, rows in ((8, 1 << 28), (384, 1 << 28), (385, 1 << 27), (768, 1 << 27), (769, 1 << 26), (4096, 1 << 26)):
+        assert lib.ea_layernorm_train(p, 0, p, p, 1e-5, o, None, None, p, rows, C, None) == -1
+        assert lib.ea_layernorm_train(p, 1, p, p, 1e-5, None, o, o, p, rows - 1, C, None) == -1
+    for C, rows in ((8, 1 << 28), (512, (1 << 28) - 15), (513, 1 << 27), (1 << 20, 1 << 17)):
+        assert lib.ea_quantize_fp8(p, 0, o, o, rows, C, None) == -1
+        assert lib.ea_dequantize_fp8(p, p, 1, o, 0, rows, C, None) == -1
+        assert lib.ea_activation_fp8(p, GELU, o, None, None, o, o, rows, C, None) == -1
+        assert lib.ea_activation_fp8_bwd(p, p, p, SILU, o, rows, C, None) == -1
+    assert lib.ea_quantize_fp8(p, 0, o, o, (1 << 62) + 5, 1 << 24, None) == -1
+    e = epilogue(a)
+    e.ldc = 1 << 22
+    for fn in (lib.ea_gemm_fp8, lib.ea_gemm_fp8_exact):
+        for kernel in KERNELS:
+            assert L.set_tuning(lib, variant=kernel) == 0
+            assert fn(p, p, p, p, 1 << 30, 1 << 22, 128, ctypes.byref(e), None) == -1
+    assert L.set_tuning(lib, variant=101) == 0
+    assert lib.ea_layernorm_bwd(p, p, 0, None, p, p, None, o, o, o, 1 << 28, 8, None, 0, None) == -1
+    lib.ea_set_tuning(None)
+    big = lib.ea_gemm_fp8_wgrad_workspace_bytes(1 << 20, 1 << 20, 1 << 20)
+    assert lib.ea_gemm_fp8_wgrad(p, p, p, o, o, 1 << 20, 1 << 20, 1 << 20, p if big else None, big, None) == -1

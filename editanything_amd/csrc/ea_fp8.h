@@ -236,5 +236,25 @@ __device__ __forceinline__ float ea_fp8_gelu(float x) {
 #define EA_FP8_ROWS (1 << 30)      // most rows of an entry that counts them in 32 bits: tile counts and row indexes stay below 2^31
 // a launch holds fewer than 2^32 threads along x
 static inline bool ea_launch_holds(long long workgroups, int threads) { return workgroups * threads < (1ll << 32); }
+// Memory of a call: n bytes at p (NULL: none).  An output may not share bytes with an input or another output; `same` allows exactly the same
+// bytes, where every element is read by the thread that writes it
+struct ea_span { const void* p; long long n; };
+static inline bool ea_apart(ea_span a, ea_span b, bool same = false) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return !x || !y || (x < y ? (long long)(y - x) >= a.n : (long long)(x - y) >= b.n) || (same && x == y && a.n == b.n);
+}
+template <size_t O, size_t I>
+static inline bool ea_outputs_apart(const ea_span (&out)[O], const ea_span (&in)[I]) {
+  for (size_t o = 0; o < O; ++o) {
+    for (size_t i = 0; i < I; ++i)
+      if (!ea_apart(out[o], in[i])) return false;
+    for (size_t i = 0; i < o; ++i)
+      if (!ea_apart(out[o], out[i])) return false;
+  }
+  return true;
+}
 static inline int ea_fp8_blocks(int cols) { return (cols + EA_FP8_BLOCK - 1) / EA_FP8_BLOCK; }
 static inline long long ea_fp8_scale_pitch(long long rows) { return (rows + 15) / 16 * 16; }
+static inline ea_span ea_codes(const void* q, long long rows, int cols) { return {q, rows * ea_fp8_blocks(cols) * EA_FP8_BLOCK}; }
+static inline ea_span ea_row_scales(const void* s, long long rows, int cols) { return {s, ea_fp8_scale_pitch(rows) * ea_fp8_blocks(cols)}; }
+static inline ea_span ea_weight_scales(const void* s, long long rows, int cols) { return {s, (rows + 127) / 128 * ea_fp8_blocks(cols)}; }

@@ -323,6 +323,7 @@ extern "C" int ea_quantize_fp8(const void* x, int in_f32, void* q, unsigned char
   const int nb = ea_fp8_blocks(cols);
   const unsigned grid = q_grid(rows, nb, gx);
   if (!grid) return EA_ERR_BAD_SHAPE;
+  if (!ea_outputs_apart({ea_codes(q, rows, cols), ea_row_scales(scale, rows, cols)}, {{x, rows * cols * (in_f32 ? 4 : 2)}})) return EA_ERR_BAD_ARG;
   const bool vec = (cols & 7) == 0 && al16(x);
   auto k = in_f32 ? (vec ? ea_quant_rows_kernel<true, true> : ea_quant_rows_kernel<true, false>)
                   : (vec ? ea_quant_rows_kernel<false, true> : ea_quant_rows_kernel<false, false>);
@@ -334,6 +335,7 @@ extern "C" int ea_quantize_fp8_weight(const void* w, int in_f32, void* q, unsign
   if (!w || !q || !scale) return EA_ERR_BAD_ARG;
   if (N <= 0 || K <= 0 || N > (1 << 22) || K > (1 << 24)) return EA_ERR_BAD_SHAPE;
   if (!al16(q)) return EA_ERR_BAD_ARG;
+  if (!ea_outputs_apart({ea_codes(q, N, K), ea_weight_scales(scale, N, K)}, {{w, (long long)N * K * (in_f32 ? 4 : 2)}})) return EA_ERR_BAD_ARG;
   const bool vec = (K & 7) == 0 && al16(w);
   auto k = in_f32 ? (vec ? ea_quant_weight_kernel<true, true> : ea_quant_weight_kernel<true, false>)
                   : (vec ? ea_quant_weight_kernel<false, true> : ea_quant_weight_kernel<false, false>);
@@ -350,6 +352,9 @@ extern "C" int ea_dequantize_fp8(const void* q, const unsigned char* scale, int 
   const int nb = ea_fp8_blocks(cols);
   const unsigned grid = q_grid(rows, nb, gx);
   if (!grid) return EA_ERR_BAD_SHAPE;
+  if (!ea_outputs_apart({{out, rows * cols * (out_f32 ? 4 : 2)}},
+                        {ea_codes(q, rows, cols), block_rows == 1 ? ea_row_scales(scale, rows, cols) : ea_weight_scales(scale, rows, cols)}))
+    return EA_ERR_BAD_ARG;
   const bool vec = (cols & 7) == 0 && al16(out);
   auto k = out_f32 ? (vec ? ea_dequant_kernel<true, true> : ea_dequant_kernel<true, false>)
                    : (vec ? ea_dequant_kernel<false, true> : ea_dequant_kernel<false, false>);
@@ -377,6 +382,13 @@ extern "C" int ea_activation_fp8(const void* z, int act, void* h, void* hq, unsi
   const int st = act_params(p, act, M, H, grid);
   if (st != EA_OK) return st;
   if (!al16(zq, hq)) return EA_ERR_BAD_ARG;
+  const int g = act == EA_ACT_GEGLU ? 2 : 1;
+  const ea_span in = {z, M * g * H * 2}, ho = {h, M * H * 2};
+  if (!ea_outputs_apart({ho, ea_codes(hq, M, H), ea_row_scales(hq ? hscale : nullptr, M, H), ea_codes(zq, g * M, H), ea_row_scales(zscale, g * M, H)},
+                        {{nullptr, 0}}) ||
+      !ea_outputs_apart({ea_codes(hq, M, H), ea_row_scales(hq ? hscale : nullptr, M, H), ea_codes(zq, g * M, H), ea_row_scales(zscale, g * M, H)}, {in}) ||
+      !ea_apart(ho, in, g == 1))
+    return EA_ERR_BAD_ARG;
   p.z = (const f16*)z; p.h = (f16*)h; p.hq = (uint8_t*)hq; p.hs = hscale; p.zq = (uint8_t*)zq; p.zs = zscale;
   const bool vec = (H & 7) == 0 && al16(z, h), o8 = hq != nullptr;
 #define EA_ACT_PICK(A) (vec ? (o8 ? ea_act_save_kernel<A, true, true> : ea_act_save_kernel<A, true, false>) \
@@ -395,6 +407,10 @@ extern "C" int ea_activation_fp8_bwd(const void* dh, const void* zq, const unsig
   const int st = act_params(p, act, M, H, grid);
   if (st != EA_OK) return st;
   if (!al16(zq)) return EA_ERR_BAD_ARG;
+  const int g = act == EA_ACT_GEGLU ? 2 : 1;
+  const ea_span out = {dz, M * g * H * 2};
+  if (!ea_outputs_apart({out}, {ea_codes(zq, g * M, H), ea_row_scales(zscale, g * M, H)}) || !ea_apart(out, {dh, M * H * 2}, g == 1))
+    return EA_ERR_BAD_ARG;
   p.dh = (const f16*)dh; p.dz = (f16*)dz; p.zq = (uint8_t*)const_cast<void*>(zq); p.zs = const_cast<unsigned char*>(zscale);
   const bool vec = (H & 7) == 0 && al16(dh, dz);
   auto k = act == EA_ACT_SILU ? (vec ? ea_act_use_kernel<EA_ACT_SILU, true> : ea_act_use_kernel<EA_ACT_SILU, false>)

@@ -802,19 +802,22 @@ WgradPlan wgrad_plan(int M, int N, int K) {
 
 long long fp8_tiles(const EaFp8GemmParams& p, int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); }
 
+// (apart: the output shares no memory with the operands; it is looked at last, behind every size)
 template <int BM, int BN, int WM, int WN, int S, bool EXACT = false>
-int fp8_ring_launch(const EaFp8GemmParams& p, void* stream) {
+int fp8_ring_launch(const EaFp8GemmParams& p, bool apart, void* stream) {
   auto k = ea_fp8_ring_kernel<BM, BN, WM, WN, S, EXACT>;
   const int smem = (BM + BN) * 128 * S + EA_F8_CH * (BM + 4);
   const long long tiles = fp8_tiles(p, BM, BN);
   if (!ea_launch_holds(tiles, 64 * WM * WN)) return EA_ERR_BAD_SHAPE;
+  if (!apart) return EA_ERR_BAD_ARG;
   ea_allow_big_lds(k, smem);
   EA_LAUNCH(k, dim3((unsigned)tiles), dim3(64 * WM * WN), smem, stream, p);
   return ea_launch_status();
 }
-int fp8_large_launch(const EaFp8GemmParams& p, void* stream) {
+int fp8_large_launch(const EaFp8GemmParams& p, bool apart, void* stream) {
   const long long tiles = fp8_tiles(p, 256, 256);
   if (!ea_launch_holds(tiles, 512)) return EA_ERR_BAD_SHAPE;
+  if (!apart) return EA_ERR_BAD_ARG;
   auto k = ea_fp8_large_kernel;
   ea_allow_big_lds(k, EA_F8L_LDS);
   EA_LAUNCH(k, dim3((unsigned)tiles), dim3(512), EA_F8L_LDS, stream, p);
@@ -830,25 +833,38 @@ int fp8_large_launch(const EaFp8GemmParams& p, void* stream) {
 //   64 x 128: from 160 tiles on.  616 x 2560 x 1024 6.7 (64 x 64: 7.5, 128 x 128: 8.5), 2048 x 1280 x 1280 9.9 (13.2, 10.0)
 //   64 x 64 with a ring of four: few tiles, where each K tile's latency counts.  512 x 1280 x 5120 15.4 (64 x 128: 23.1),
 //       77 x 1024 x 1024 6.1 (6.0)
-int fp8_launch(EaFp8GemmParams& p, void* stream) {
+int fp8_launch(EaFp8GemmParams& p, bool apart, void* stream) {
   p.raster_gm = 8;                         // (4 and 16: within 2 %)
   const int v = ea_forced_variant();
   const long long large = fp8_tiles(p, 256, 256), rounds = (large + 255) / 256;
-  if (v == 101 || (v < 101 && p.nb >= 8 && large * 4 >= rounds * 256 * 3)) return fp8_large_launch(p, stream);
-  if (v == 102 || (v < 101 && fp8_tiles(p, 128, 128) >= 256)) return fp8_ring_launch<128, 128, 2, 4, 2>(p, stream);
-  if (v == 103 || (v < 101 && fp8_tiles(p, 64, 128) >= 160)) return fp8_ring_launch<64, 128, 2, 4, 2>(p, stream);
-  return fp8_ring_launch<64, 64, 2, 2, 4>(p, stream);
+  if (v == 101 || (v < 101 && p.nb >= 8 && large * 4 >= rounds * 256 * 3)) return fp8_large_launch(p, apart, stream);
+  if (v == 102 || (v < 101 && fp8_tiles(p, 128, 128) >= 256)) return fp8_ring_launch<128, 128, 2, 4, 2>(p, apart, stream);
+  if (v == 103 || (v < 101 && fp8_tiles(p, 64, 128) >= 160)) return fp8_ring_launch<64, 128, 2, 4, 2>(p, apart, stream);
+  return fp8_ring_launch<64, 64, 2, 2, 4>(p, apart, stream);
 }
 // The same with exact products (the 8-bit kernels' time behind it): 128 x 128 from 512 tiles on: 16384 x 5120 x 1280 252 us (64 x 128: 292, 64 x 64:
 // 369; 111), 32768 x 320 x 320 18.2 (19.9, 23.9; 12.1), 8192^3 1029 = 1070 TFLOP/s (390); but 8192 x 640 x 640, 320 tiles, 17.0 (15.4, 18.0; 10.2).
 // 64 x 128 from 160 tiles on: 616 x 2560 x 1024 9.7 (64 x 64: 10.6; 6.6), 2048 x 1280 x 1280 16.5 (17.8; 9.6).  64 x 64 below: 512 x 1280 x
 // 5120 25.5 (64 x 128: 31.5; 15.0).
-int fp8_exact_launch(EaFp8GemmParams& p, void* stream) {
+int fp8_exact_launch(EaFp8GemmParams& p, bool apart, void* stream) {
   p.raster_gm = 8;
   const int v = ea_forced_variant();
-  if (v == 102 || (v < 101 && fp8_tiles(p, 128, 128) >= 512)) return fp8_ring_launch<128, 128, 2, 2, 2, true>(p, stream);
-  if (v == 103 || (v < 101 && fp8_tiles(p, 64, 128) >= 160)) return fp8_ring_launch<64, 128, 2, 4, 2, true>(p, stream);
-  return fp8_ring_launch<64, 64, 2, 2, 4, true>(p, stream);
+  if (v == 102 || (v < 101 && fp8_tiles(p, 128, 128) >= 512)) return fp8_ring_launch<128, 128, 2, 2, 2, true>(p, apart, stream);
+  if (v == 103 || (v < 101 && fp8_tiles(p, 64, 128) >= 160)) return fp8_ring_launch<64, 128, 2, 4, 2, true>(p, apart, stream);
+  return fp8_ring_launch<64, 64, 2, 2, 4, true>(p, apart, stream);
+}
+
+// rows of `width` bytes, `pitch` apart, against other memory: rows of the same pitch, or one piece (pitch 0)
+struct RowSpan { const void* p; long long rows, pitch, width; };
+bool rows_apart(const RowSpan& a, const RowSpan& b) {
+  const ea_span x = {a.p, (a.rows - 1) * a.pitch + a.width}, y = {b.p, (b.rows - 1) * b.pitch + b.width};
+  if (ea_apart(x, y)) return true;
+  if (b.pitch && b.pitch != a.pitch) return false;
+  const RowSpan& lo = (uintptr_t)a.p <= (uintptr_t)b.p ? a : b;
+  const RowSpan& hi = &lo == &a ? b : a;
+  if (!lo.pitch) return false;
+  const long long d = (long long)((uintptr_t)hi.p - (uintptr_t)lo.p) % lo.pitch;         // beside lo's columns?
+  return d >= lo.width && d + hi.width <= lo.pitch;
 }
 
 int gemm_fp8_entry(const void* a, const unsigned char* a_scale, const void* w, const unsigned char* w_scale, int M, int N, int K, const ea_epilogue* e,
@@ -870,7 +886,14 @@ int gemm_fp8_entry(const void* a, const unsigned char* a_scale, const void* w, c
   p.vec = (N & 7) == 0 && (e->ldc & 7) == 0 && e->ldc < (1 << 21) && ((uintptr_t)e->out & 15) == 0;
   if (e->residual || e->residual32)
     p.vec = p.vec && (e->ldr & 7) == 0 && e->ldr < (1 << 21) && ((((uintptr_t)e->residual) | ((uintptr_t)e->residual32)) & 15) == 0;
-  return exact ? fp8_exact_launch(p, stream) : fp8_launch(p, stream);
+  const int es = e->out_f32 ? 4 : 2, rs = e->residual32 ? 4 : 2;
+  const RowSpan out = {e->out, M, (long long)e->ldc * es, (long long)N * es};
+  const void* const res = e->residual32 ? (const void*)e->residual32 : e->residual;
+  bool apart = true;
+  for (const ea_span& in : {ea_codes(a, M, K), ea_row_scales(a_scale, M, K), ea_codes(w, N, K), ea_weight_scales(w_scale, N, K), ea_span{e->bias, 4ll * N}})
+    apart = apart && rows_apart(out, {in.p, 1, 0, in.n});
+  if (res && !(res == e->out && rs == es && e->ldr == e->ldc)) apart = apart && rows_apart(out, {res, M, (long long)e->ldr * rs, (long long)N * rs});
+  return exact ? fp8_exact_launch(p, apart, stream) : fp8_launch(p, apart, stream);
 }
 
 }  // namespace
@@ -913,6 +936,9 @@ extern "C" int ea_gemm_fp8_wgrad(const void* dy, const void* x, const unsigned c
   const long long tiles = (long long)p.tiles_n * p.tiles_k;
   const long long total = (long long)N * K + N;
   if (!ea_launch_holds(tiles, 512) || (p.splits > 1 && !ea_launch_holds((total + 255) / 256, 64))) return EA_ERR_BAD_SHAPE;
+  if (!ea_outputs_apart({{dw, 4ll * N * K}, {db, 4ll * N}, {p.splits > 1 ? workspace : nullptr, p.splits * p.part * 4}},
+                        {{dy, 2ll * M * N}, ea_codes(x, M, K), ea_row_scales(x_scale, M, K)}))
+    return EA_ERR_BAD_ARG;
   if (kernel == 256) {
     auto k = ea_fp8_wgrad_large_kernel;
     ea_allow_big_lds(k, WL_LDS);

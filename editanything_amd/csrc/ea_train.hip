@@ -441,15 +441,18 @@ bool ln_vec(int C, const void* a, const void* b, const void* c, const void* d, c
   return (C & 7) == 0 && ((((uintptr_t)a) | ((uintptr_t)b) | ((uintptr_t)c) | ((uintptr_t)d) | ((uintptr_t)e) | ((uintptr_t)f)) & 15) == 0;
 }
 int ln_lanes(int C) { return C <= 384 ? 16 : C <= 768 ? 32 : 64; }       // lanes per row
+long long ln_row_groups(int M, int C) {                                  // workgroups that hold a row per group of lanes
+  const int rows = 4 * (64 / ln_lanes(C));
+  return ((long long)M + rows - 1) / rows;
+}
 
 template <int XK, bool ANY, bool OUT8>
 int ln_train_launch(const LnTrainParams& p, void* stream) {
-  const int lpr = ln_lanes(p.C), rows = 4 * (64 / lpr);
-  if (!ea_launch_holds((p.M + rows - 1) / rows, 256)) return EA_ERR_BAD_SHAPE;
+  const int lpr = ln_lanes(p.C);
   auto k = lpr == 16 ? ea_ln_train_kernel<XK, ANY, 16, 3, OUT8> : lpr == 32 ? ea_ln_train_kernel<XK, ANY, 32, 3, OUT8>
          : p.C <= 1536 ? ea_ln_train_kernel<XK, ANY, 64, 3, OUT8> : p.C <= 2560 ? ea_ln_train_kernel<XK, ANY, 64, 5, OUT8>
          : ea_ln_train_kernel<XK, ANY, 64, 8, OUT8>;
-  EA_LAUNCH(k, dim3((p.M + rows - 1) / rows), dim3(256), 0, stream, p);
+  EA_LAUNCH(k, dim3((unsigned)ln_row_groups(p.M, p.C)), dim3(256), 0, stream, p);
   return ea_launch_status();
 }
 template <int XK>
@@ -461,10 +464,9 @@ int ln_train_pick(const LnTrainParams& p, bool vec, void* stream) {
 // Workgroups of the backward pass: as many as are resident (two per CU up to 1536 columns, one above), each walking the rows.  us for
 // 256 / 512 / 1024: 32768 x 320 23.1 / 22.8 / 28.3, 32768 x 1280 47.8 / 45.1 / 49.2, 4096 x 4096 34.9 / 43.1 / 60.9.
 int ln_bwd_grid(int M, int C) {
-  const int rows = 4 * (64 / ln_lanes(C));
-  const int g = (M + rows - 1) / rows;
+  const long long g = ln_row_groups(M, C);
   const int most = C > 1536 ? 256 : 512;
-  return g < most ? g : most;
+  return g < most ? (int)g : most;
 }
 
 // One launch (ea_ln_bwd_few_kernel)?  us, one launch / two: 1 x 1280 2.5 / 6.7, 512 x 1280 3.7 / 8.5, 616 x 1024 in 8 bits 4.2 / 8.5, 1024 x 1280
@@ -477,12 +479,11 @@ bool ln_bwd_few(int M) {
 
 template <int XK, bool F32, bool ANY>
 int ln_bwd_few_launch(const LnBwdParams& p, float* dgamma, float* dbeta, void* stream) {
-  const int lpr = ln_lanes(p.C), rows = 4 * (64 / lpr), ncol = (p.C + LF_COLS - 1) / LF_COLS;
-  if (!ea_launch_holds(ncol + (long long)(p.M + rows - 1) / rows, 256)) return EA_ERR_BAD_SHAPE;
+  const int lpr = ln_lanes(p.C), ncol = (p.C + LF_COLS - 1) / LF_COLS;
   auto k = lpr == 16 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 16, 3> : lpr == 32 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 32, 3>
          : p.C <= 1536 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 3> : p.C <= 2560 ? ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 5>
          : ea_ln_bwd_few_kernel<XK, F32, ANY, 64, 8>;
-  EA_LAUNCH(k, dim3(ncol + (p.M + rows - 1) / rows), dim3(256), LF_LDS, stream, p, dgamma, dbeta, ncol);
+  EA_LAUNCH(k, dim3((unsigned)(ncol + ln_row_groups(p.M, p.C))), dim3(256), LF_LDS, stream, p, dgamma, dbeta, ncol);
   return ea_launch_status();
 }
 
@@ -507,8 +508,13 @@ int ln_bwd_pick(const LnBwdParams& p, bool vec, int grid, float* dgamma, float* 
 extern "C" int ea_layernorm_train(const void* x, int in_f32, const float* gamma, const float* beta, float eps, void* y, void* q,
                                   unsigned char* scale, float* stats, int M, int C, void* stream) {
   if (!x || !gamma || !beta || !stats || (!y == !q) || (q && !scale)) return EA_ERR_BAD_ARG;
-  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
+  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096 || !ea_launch_holds(ln_row_groups(M, C), 256)) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)stats & 7) || ((uintptr_t)q & 15)) return EA_ERR_BAD_ARG;
+  const ea_span in = {x, (long long)M * C * (in_f32 ? 4 : 2)}, yo = {y, (long long)M * C * 2}, st = {stats, 8ll * M};
+  const ea_span ga = {gamma, 4ll * C}, be = {beta, 4ll * C};
+  if (!ea_outputs_apart({yo, ea_codes(q, M, C), ea_row_scales(q ? scale : nullptr, M, C), st}, {ga, be}) ||
+      !ea_outputs_apart({ea_codes(q, M, C), ea_row_scales(q ? scale : nullptr, M, C), st}, {in}) || !ea_apart(yo, in, true))
+    return EA_ERR_BAD_ARG;
   LnTrainParams p;
   p.x = x; p.gamma = gamma; p.beta = beta; p.y = (f16*)y; p.q = (uint8_t*)q; p.scale = scale; p.stats = stats;
   p.M = M; p.C = C; p.Kp = ea_fp8_blocks(C) * EA_FP8_BLOCK; p.Rp = ea_fp8_scale_pitch(M); p.eps = eps;
@@ -529,7 +535,15 @@ extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const
   if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)stats & 7) || ((uintptr_t)workspace & 3)) return EA_ERR_BAD_ARG;
   const bool few = ln_bwd_few(M);
+  if (few && !ea_launch_holds(ln_row_groups(M, C) + (C + LF_COLS - 1) / LF_COLS, 256)) return EA_ERR_BAD_SHAPE;
   if (!few && (!workspace || ws_bytes < ea_layernorm_bwd_workspace_bytes(M, C))) return EA_ERR_WORKSPACE;
+  const long long es = x_kind == XK_F32 ? 4 : 2, n = (long long)M * C;
+  const ea_span xs = x_kind == XK_FP8 ? ea_codes(x, M, C) : ea_span{x, n * es}, out = {dx, n * es};
+  const ea_span wk = {few ? nullptr : workspace, (long long)ea_layernorm_bwd_workspace_bytes(M, C)};
+  if (!ea_outputs_apart({out, {dgamma, 4ll * C}, {dbeta, 4ll * C}, wk},
+                        {{dy, 2 * n}, xs, ea_row_scales(x_kind == XK_FP8 ? x_scale : nullptr, M, C), {stats, 8ll * M}, {gamma, 4ll * C}}) ||
+      !ea_outputs_apart({{dgamma, 4ll * C}, {dbeta, 4ll * C}, wk}, {{residual, n * es}}) || !ea_apart(out, {residual, n * es}, true))
+    return EA_ERR_BAD_ARG;
   LnBwdParams p;
   p.dy = (const f16*)dy; p.x = x; p.x_scale = x_scale; p.stats = stats; p.gamma = gamma; p.residual = residual; p.dx = dx;
   p.part = (float*)workspace; p.M = M; p.C = C;

@@ -1262,10 +1262,15 @@ def gemm_fp8(a, w, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=t
             and (out is None or (out.dtype in (_F16, _F32) and out.shape == shape))):
         _refuse(f"gemm_fp8: bias must be fp32 [{N}], residual and out fp16 or fp32 {shape}", bias=bias, residual=residual, out=out,
                 out_dtype=out_dtype)
-    if out is not None and residual is not None:
-        po, pr = out.data_ptr(), residual.data_ptr()
-        if (po != pr or out.dtype != residual.dtype) and po < pr + residual.nbytes and pr < po + out.nbytes:
-            _refuse("gemm_fp8: residual has to be out or lie apart from it", residual=residual, out=out)
+    if out is not None:
+        po, end = out.data_ptr(), out.data_ptr() + out.nbytes
+        if residual is not None:
+            pr = residual.data_ptr()
+            if (po != pr or out.dtype != residual.dtype) and po < pr + residual.nbytes and pr < end:
+                _refuse("gemm_fp8: residual has to be out or lie apart from it", residual=residual, out=out)
+        for t in (a.q, a.scale, w.q, w.scale, bias):
+            if t is not None and po < t.data_ptr() + t.nbytes and t.data_ptr() < end:
+                _refuse("gemm_fp8: out has to lie apart from the operands", out=out, operand=t)
     _on_device(dev, a.q, a.scale, w.q, w.scale, bias, residual, out)
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=dev)

@@ -409,6 +409,8 @@ int ea_add_f16(const void* a, const void* b, void* out, long long n, void* strea
  * Entries that take the rows as an int take at most 2^30, and every entry what one launch of fewer than 2^32 threads covers: LayerNorm
  * forward 2^28 - 16 rows of up to 384 columns, 2^27 - 8 of up to 768, 2^26 - 4 of more; quantisation, its inverse and the activations
  * 2^28 - 16 rows of up to 512 columns, and so on in proportion (EA_ERR_BAD_SHAPE).
+ * Outputs and workspaces share no bytes with inputs or each other (EA_ERR_BAD_ARG).  Exactly the same memory is allowed for z and h, dh and dz (SiLU,
+ * GELU), x and y of one type (LayerNorm forward), residual and dx, residual and out of one type and pitch.
  * ea_quantize_fp8 / ea_quantize_fp8_weight: x / w fp16 (in_f32 = 0) or fp32, dense rows.
  * ea_dequantize_fp8: block_rows = 1 (rows) or 128 (weight); out dense fp16 or fp32. */
 int ea_quantize_fp8(const void* x, int in_f32, void* q, unsigned char* scale, long long rows, int cols, void* stream);

@@ -285,3 +285,65 @@ def test_more_than_a_launch_holds_is_refused(emu_lib):
     lib.ea_set_tuning(None)
     big = lib.ea_gemm_fp8_wgrad_workspace_bytes(1 << 20, 1 << 20, 1 << 20)
     assert lib.ea_gemm_fp8_wgrad(p, p, p, o, o, 1 << 20, 1 << 20, 1 << 20, p if big else None, big, None) == -1
+
+
+def test_outputs_that_share_memory_with_inputs_are_refused(emu_lib):
+    """Which thread reads an element before which writes it is no caller's business: the C entries refuse what they cannot get right, and take
+    the in-place calls that they can."""
+    lib = emu_lib
+    m = np.zeros(1 << 20, np.uint8)
+    at = lambda kib: m.ctypes.data + 1024 * kib  # noqa: E731
+    # LayerNorm backward: up to 1024 rows the column sums read all of x and dy beside the writers of dx
+    bwd = lambda dy=0, x=100, dx=200, res=None, st=300, ga=310, dg=320, db=330, kind=0, M=64: lib.ea_layernorm_bwd(  # noqa: E731
+        at(dy), at(x), kind, at(500) if kind == 2 else None, at(st), at(ga), None if res is None else at(res), at(dx), at(dg), at(db), M, 64, at(400), 1 << 20,
+        None)
+    assert bwd() == bwd(res=200) == bwd(kind=1) == bwd(kind=2) == bwd(dx=8) == bwd(dx=108) == 0          # (64 rows of 64: 8 KiB)
+    assert bwd(dx=0) == bwd(dx=7) == bwd(dx=100) == bwd(dx=99) == bwd(dx=200, res=201) == bwd(dg=101) == bwd(dg=330) == bwd(db=200) == -2
+    assert bwd(dx=100, kind=1) == bwd(dx=200, res=207) == bwd(ga=200) == bwd(st=201) == bwd(kind=2, dx=500) == -2
+    fwd = lambda x=0, y=100, q=None, st=300, f32=0, ga=310: lib.ea_layernorm_train(  # noqa: E731
+        at(x), f32, at(ga), at(320), 1e-5, at(y) if q is None else None, None if q is None else at(q), at(200), at(st), 64, 64, None)
+    assert fwd() == fwd(y=0) == fwd(q=100) == fwd(f32=1) == 0
+    assert fwd(y=0, f32=1) == fwd(y=7) == fwd(q=0) == fwd(q=200) == fwd(st=0) == fwd(st=100) == fwd(ga=100) == -2
+    act = lambda fn, z=0, h=100, zq=200, zs=300: lib.ea_activation_fp8(at(z), fn, at(h), None, None, at(zq), at(zs), 64, 64, None)  # noqa: E731
+    assert act(GELU) == act(GELU, h=0) == act(GEGLU) == 0
+    assert act(GEGLU, h=0) == act(GELU, h=1) == act(GELU, zq=0) == act(GELU, zs=100) == act(SILU, zs=200) == -2
+    assert lib.ea_activation_fp8(at(0), SILU, None, at(0), at(300), at(200), at(310), 64, 64, None) == -2
+    use = lambda fn, dh=0, dz=100, zq=200, zs=300: lib.ea_activation_fp8_bwd(at(dh), at(zq), at(zs), fn, at(dz), 64, 64, None)  # noqa: E731
+    assert use(GELU) == use(SILU, dz=0) == use(GEGLU) == 0
+    assert use(GEGLU, dz=0) == use(GELU, dz=1) == use(GELU, dz=200) == use(GELU, dz=300) == -2
+    assert lib.ea_quantize_fp8(at(0), 0, at(4), at(300), 64, 64, None) == lib.ea_quantize_fp8(at(0), 0, at(100), at(100), 64, 64, None) == -2
+    assert lib.ea_quantize_fp8_weight(at(0), 1, at(15), at(300), 64, 64, None) == lib.ea_quantize_fp8_weight(at(0), 0, at(8), at(0), 64, 64, None) == -2
+    assert lib.ea_dequantize_fp8(at(0), at(300), 1, at(7), 0, 64, 64, None) == lib.ea_dequantize_fp8(at(0), at(300), 128, at(300), 1, 64, 64, None) == -2
+
+    # the product: 64 x 64 fp16 outputs (8 KiB), a at 0, its scales at 20, w at 40, its scales at 60, bias at 80
+    def mm(fn, out=100, res=None, res32=None, ldc=64, ldr=64, f32=0, more=0):
+        e = L.Epilogue()
+        e.bias, e.scale, e.out, e.ldc, e.out_f32, e.ldr = at(80), 1.0, at(out), ldc, f32, ldr
+        if res is not None:
+            e.residual = at(res) + more
+        if res32 is not None:
+            e.residual32 = at(res32)
+        return fn(at(0), at(20), at(40), at(60), 64, 64, 64, ctypes.byref(e), None)
+    for fn in (lib.ea_gemm_fp8, lib.ea_gemm_fp8_exact):
+        assert mm(fn) == mm(fn, res=100) == mm(fn, res=108) == mm(fn, res=92) == mm(fn, f32=1, res32=100) == 0
+        assert mm(fn, ldc=128, ldr=128, res=100, more=128) == 0                 # two halves of one buffer's rows
+        assert mm(fn, ldc=128, ldr=128, res=100, more=126) == mm(fn, ldc=128, ldr=128, res=100, more=130) == mm(fn, ldc=128, res=100) == -2
+        assert mm(fn, res=101) == mm(fn, res=99) == mm(fn, res32=100) == mm(fn, f32=1, res=100) == mm(fn, res32=90) == -2
+        assert mm(fn, out=4) == mm(fn, out=13) == mm(fn, out=40) == mm(fn, out=53) == mm(fn, out=60) == mm(fn, out=80) == -2
+    wg = lambda dy=0, x=100, dw=200, db=300, ws=400, M=64: lib.ea_gemm_fp8_wgrad(at(dy), at(x), at(700), at(dw), at(db), M, 64, 64, at(ws), 1 << 20,  # noqa: E731
+                                                                                None)
+    assert wg() == 0
+    assert wg(dw=0) == wg(dw=107) == wg(dw=700) == wg(db=200) == wg(db=100) == -2
+    assert lib.ea_gemm_fp8_wgrad_workspace_bytes(700, 64, 64) > 0 and wg(M=700) == 0
+    assert wg(M=700, ws=200) == wg(M=700, ws=80) == wg(M=700, ws=290) == -2
+
+
+def test_gemm_fp8_refuses_an_output_that_is_an_operand():
+    t = ops.Fp8Tensor(torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(1, 16, dtype=torch.uint8), 8)
+    w = ops.Fp8Tensor(torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(1, 1, dtype=torch.uint8), 8)
+    b = torch.zeros(32)
+    for out, bias in ((t.q.view(torch.float16)[0, :16].view(4, 4), None), (w.q.view(torch.float32)[3, 16:].view(4, 4), None), (b[:16].view(4, 4), b[12:16])):
+        with pytest.raises(ValueError, match="apart"):
+            ops.gemm_fp8(t, w, out=out, bias=bias)
+    with pytest.raises(RuntimeError, match="MI355X"):               # accepted: on the CPU only the missing device stops it
+        ops.gemm_fp8(t, w, out=b[:16].view(4, 4), bias=b[16:20])

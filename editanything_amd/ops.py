@@ -1022,7 +1022,8 @@ def add_f16(a, b):
 # ------------------------------------------------------------------------------------------------ 8-bit training operators
 # LayerNorm with its backward pass, activations whose input is kept in 8 bits for the backward pass, the product of 8-bit operands and
 # the weight gradient from an 8-bit input: what a transformer block (LayerNorm -> Linear -> activation -> Linear + residual) needs to be
-# trained with its activations held in 8 bits.  Every operator is a plain function; the caller keeps what the backward pass takes.
+# trained with its activations held in 8 bits.  Every operator is a plain function; the caller keeps what the backward pass takes.  None records an
+# autograd graph: where one is being recorded, an operand that requires grad is refused (its gradient would be cut off without a word).
 # Outputs and scratch come from torch's allocator on the current stream of the operands' device, never from the shared per-thread
 # workspace, so calls on several streams and in several captured graphs do not meet.
 FP8_BLOCK = 128
@@ -1044,7 +1045,12 @@ def _refuse(rule, **given):
 
 
 def _on_device(dev, *tensors):
-    """All operands dense and on one MI355X."""
+    """All operands dense and on one MI355X, and none that a recorded graph would have to know of."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the 8-bit training operators record no autograd graph, and an operand requires grad: call them under torch.no_grad() or from "
+                                   "an autograd.Function, and their backward operators from its backward pass")
     if dev.type != "cuda":
         raise RuntimeError(f"editanything_amd ops run on the MI355X only (an operand is on {dev})")
     for t in tensors:
@@ -1272,7 +1278,8 @@ def gemm_fp8(a, w, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=t
             if t is not None and po < t.data_ptr() + t.nbytes and t.data_ptr() < end:
                 _refuse("gemm_fp8: out has to lie apart from the operands", out=out, operand=t)
     _on_device(dev, a.q, a.scale, w.q, w.scale, bias, residual, out)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(shape, dtype=out_dtype, device=dev)
     if M:
         e = L.Epilogue()
@@ -1286,6 +1293,8 @@ def gemm_fp8(a, w, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=t
         lib = _lib()
         fn = lib.ea_gemm_fp8_exact if (out.dtype == _F32 if exact is None else exact) else lib.ea_gemm_fp8
         _run(dev, "ea_gemm_fp8", fn, a.q.data_ptr(), a.scale.data_ptr(), w.q.data_ptr(), w.scale.data_ptr(), M, N, a.cols, C.byref(e))
+        if given and not out.is_inference():
+            torch.autograd.graph.increment_version(out)        # (a graph that has saved `out` finds out)
     return out
 
 

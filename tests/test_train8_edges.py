@@ -347,3 +347,70 @@ def test_gemm_fp8_refuses_an_output_that_is_an_operand():
             ops.gemm_fp8(t, w, out=out, bias=bias)
     with pytest.raises(RuntimeError, match="MI355X"):               # accepted: on the CPU only the missing device stops it
         ops.gemm_fp8(t, w, out=b[:16].view(4, 4), bias=b[16:20])
+
+
+def test_an_operand_that_requires_grad_is_refused_where_a_graph_is_recorded():
+    x, one, zero = torch.zeros(4, 8, dtype=torch.float16), torch.ones(8), torch.zeros(4, 2)
+    q, sc = torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(1, 16, dtype=torch.uint8)
+    t, w = ops.Fp8Tensor(q, sc, 8), ops.Fp8Tensor(q, torch.zeros(1, 1, dtype=torch.uint8), 8)
+    gx, gone = x.clone().requires_grad_(), one.clone().requires_grad_()
+    calls = [lambda: ops.quantize_fp8(gx), lambda: ops.quantize_fp8_weight(gx), lambda: ops.layernorm_train(gx, one, one),
+             lambda: ops.layernorm_train(x, gone, one), lambda: ops.layernorm_train(x, one, gone), lambda: ops.layernorm_backward(gx, x, zero, one),
+             lambda: ops.layernorm_backward(x, x, zero, gone), lambda: ops.layernorm_backward(x, x, zero, one, residual=gx),
+             lambda: ops.activation_fp8(gx, ops.ACT_GELU), lambda: ops.activation_fp8_backward(gx, t, ops.ACT_GELU),
+             lambda: ops.gemm_fp8(t, w, bias=torch.zeros(4, requires_grad=True)), lambda: ops.gemm_fp8(t, w, residual=gx[:, :4].contiguous()),
+             lambda: ops.gemm_fp8(t, w, out=torch.zeros(4, 4, requires_grad=True)), lambda: ops.gemm_fp8_wgrad(gx, t)]
+    for f in calls:
+        with pytest.raises(RuntimeError, match="autograd"):
+            f()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="MI355X"):      # accepted: on the CPU only the missing device stops it
+            f()
+
+
+@pytest.mark.gpu
+def test_training_operators_inside_an_autograd_function():
+    """A LayerNorm and a Linear in 8 bits as an autograd.Function's forward and backward pass; a written `out` is noticed by a graph that saved it."""
+    g = torch.Generator(device="cuda").manual_seed(45)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+
+    class Block(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, gamma, beta, w, b):
+            n, stats = ops.layernorm_train(x, gamma, beta, fp8=True)
+            ctx.save_for_backward(x, gamma, stats, w)
+            ctx.n = n
+            return ops.gemm_fp8(n, ops.quantize_fp8_weight(w), bias=b)
+
+        @staticmethod
+        def backward(ctx, dy):
+            x, gamma, stats, w = ctx.saved_tensors
+            dw, db = ops.gemm_fp8_wgrad(dy, ctx.n)
+            dn = ops.gemm_fp8(ops.quantize_fp8(dy), ops.quantize_fp8_weight(w.t().contiguous()))
+            return ops.layernorm_backward(dn, x, stats, gamma) + (dw, db)
+    p = [r(77, 320).half(), 1 + 0.2 * r(320), 0.1 * r(320), r(640, 320) * 320 ** -0.5, 0.1 * r(640)]
+    leaves = [t.clone().requires_grad_() for t in p]
+    dy = (0.02 * r(77, 640)).half()
+    got = torch.autograd.grad(Block.apply(*leaves), leaves, dy)
+
+    class Ctx:
+        def save_for_backward(self, *t):
+            self.saved_tensors = t
+    with torch.no_grad():
+        ctx = Ctx()
+        Block.forward(ctx, *p)
+        ref = Block.backward(ctx, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    # ... and they are gradients: of the function in fp32, to what 8-bit operands give (each within 2^-4 of its value, signs random)
+    m = [t.clone().float().requires_grad_() for t in p]
+    out = torch.nn.functional.linear(torch.nn.functional.layer_norm(m[0], (320,), m[1], m[2]), m[3], m[4])
+    for a, b in zip(got, torch.autograd.grad(out, m, dy.float())):
+        assert (a.float() - b).norm() <= 2.0 ** -4 * b.norm()
+    a, w = ops.quantize_fp8(p[0]), ops.quantize_fp8_weight(p[3])
+    y = torch.zeros(77, 640, device="cuda", dtype=torch.float16)
+    z = torch.ones(77, 640, device="cuda", dtype=torch.float16, requires_grad=True)
+    prod = z * y
+    ops.gemm_fp8(a, w, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        prod.sum().backward()
+    with torch.inference_mode():
+        ops.gemm_fp8(a, w, out=torch.zeros(77, 640, device="cuda", dtype=torch.float16))

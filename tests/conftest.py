@@ -32,6 +32,7 @@ def pytest_collection_modifyitems(config, items):
         items[:] = keep
 
 
+@pytest.hookimpl(trylast=True)           # behind the runner's own hook, which tears the module's fixtures down
 def pytest_runtest_teardown(item, nextitem):
     """Dead cycles of a module's fixtures (captured graphs among them) go between modules, not inside a later test's own graph capture,
     where the destructor of a graph ends the process (ops.graph_capture)."""

@@ -32,10 +32,12 @@ def pytest_collection_modifyitems(config, items):
         items[:] = keep
 
 
-@pytest.hookimpl(trylast=True)           # behind the runner's own hook, which tears the module's fixtures down
-def pytest_runtest_teardown(item, nextitem):
+@pytest.hookimpl(hookwrapper=True)
+def pytest_runtest_protocol(item, nextitem):
     """Dead cycles of a module's fixtures (captured graphs among them) go between modules, not inside a later test's own graph capture,
-    where the destructor of a graph ends the process (ops.graph_capture)."""
+    where the destructor of a graph ends the process (ops.graph_capture).  Behind the whole of the module's last test: while it is being torn
+    down, it still holds its fixtures."""
+    yield
     if nextitem is None or getattr(nextitem, "module", None) is not getattr(item, "module", None):
         import gc
         gc.collect()

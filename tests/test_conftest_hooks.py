@@ -14,7 +14,7 @@ def test_a_modules_fixtures_are_collected_before_the_next_module(tmp_path):
         spec = importlib.util.spec_from_file_location("hooks", {hooks!r})
         hooks = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(hooks)
-        globals().update({n: f for n, f in vars(hooks).items() if n.startswith("pytest_runtest")})
+        globals().update({{n: f for n, f in vars(hooks).items() if n.startswith("pytest_runtest")}})
         gc.disable()
         refs = []
         """))

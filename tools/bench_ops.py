@@ -10,7 +10,7 @@ import sys
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-from editanything_amd import _lib as L  # noqa: E402
+from editanything_amd import _lib as L, ops  # noqa: E402
 
 PEAK_TF, PEAK_GBS = 2500.0, 8000.0
 lib = L.lib()
@@ -30,7 +30,7 @@ def timeit(fn, iters=20, warm=3):
         fn()
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
+    with ops.graph_capture(g):
         for _ in range(iters):
             fn()
     g.replay()

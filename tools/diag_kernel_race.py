@@ -213,7 +213,7 @@ def step1():
             run()
         torch.cuda.current_stream().wait_stream(s)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with ops.graph_capture(graph):
             gout = run()
         graph.replay()
         torch.cuda.synchronize()

@@ -51,7 +51,7 @@ for spec in (sys.argv[1:] or ["base"]):
             out = run()
         torch.cuda.current_stream().wait_stream(s)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with ops.graph_capture(graph):
             out = run()
         for _ in range(3):
             graph.replay()

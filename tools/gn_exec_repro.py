@@ -89,7 +89,7 @@ for name in LIBS:
             run()
         torch.cuda.current_stream().wait_stream(s)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with ops.graph_capture(graph):
             gout = run()
         graph.replay()
         torch.cuda.synchronize()

@@ -39,7 +39,7 @@ def capture(slot, tag, stream):
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
     with torch.cuda.stream(stream):
-        with torch.cuda.graph(g, stream=stream):
+        with ops.graph_capture(g, stream=stream):
             work(slot, tag)
     torch.cuda.synchronize()
     return g

@@ -28,7 +28,7 @@ def worker(i, concurrent):
             run = lambda: den.eps(lat, ts, embs=embs, cfg_halves=True, cfg_single=True)
             run(); torch.cuda.synchronize()
             graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+            with ops.graph_capture(graph, stream=s, capture_error_mode="thread_local"):
                 out = run()
             graph.replay(); torch.cuda.synchronize()
             ref = out.clone()

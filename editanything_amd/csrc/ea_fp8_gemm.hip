@@ -773,11 +773,16 @@ struct WgradPlan { int kernel, splits, rows; };
 WgradPlan wgrad_plan(int M, int N, int K) {
   WgradPlan w{-1, 1, 64};
   const int v = ea_forced_variant();       // tests: 101, 102, 103 pin a kernel
-  const int f = ea_forced_splits() < (M + 63) / 64 ? ea_forced_splits() : 0;
   const bool large = K > 256;              // (two k tiles: each sums one half of its dy columns for db)
   const bool dma = (N & 7) == 0 && N <= (1 << 18) && K <= (1 << 18) && v != 103;
   const double nk = (double)N * K;
   const int steps = (M + 63) / 64;
+  int f = ea_forced_splits();              // tests: this many slices, where that leaves none empty
+  if (f < 1 || f > steps || f > 64) f = 0;
+  if (f) {
+    const int per = (steps + f - 1) / f;
+    if ((steps + per - 1) / per != f) f = 0;
+  }
   double best = 0;
   for (int kernel = 256; kernel >= 0; kernel -= 128) {
     if (kernel ? !dma || (kernel == 256 ? !large || v == 102 : large && v == 101) : dma) continue;

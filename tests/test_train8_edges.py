@@ -414,3 +414,21 @@ def test_training_operators_inside_an_autograd_function():
         prod.sum().backward()
     with torch.inference_mode():
         ops.gemm_fp8(a, w, out=torch.zeros(77, 640, device="cuda", dtype=torch.float16))
+
+
+# ------------------------------------------------------------------------------------------------------------- launch rules
+def test_pinned_slices_that_would_leave_one_empty_are_not_taken(emu_lib):
+    M, N, K = 600, 24, 100                                     # ten steps: 6, 7, 8 and 9 slices would leave some empty
+    q, e = quantize(rows(46, M, K, np.float32))
+    dy = rows(47, M, N, np.float16, 0.05)
+    d, x = dy.astype(np.float64), values(q, e, K)
+    for splits in (1, 2, 3, 6, 9, 10, 11, 65, -1):
+        assert L.set_tuning(emu_lib, splits=splits) == 0
+        nbytes = emu_lib.ea_gemm_fp8_wgrad_workspace_bytes(M, N, K)
+        if splits in (1, 2, 10):
+            assert nbytes == (0 if splits == 1 else 4 * splits * (N * K + N))
+        dw, db, ws = np.zeros((N, K), np.float32), np.zeros(N, np.float32), np.zeros(max(nbytes // 4, 4), np.float32)
+        st = emu_lib.ea_gemm_fp8_wgrad(ptr(dy), ptr(q), ptr(pack_scales(e)), ptr(dw), ptr(db), M, N, K, ptr(ws) if nbytes else None, nbytes, None)
+        emu_lib.ea_set_tuning(None)
+        assert st == 0 and (np.abs(dw - d.T @ x) <= 2 * (M + 2) * U32 * (np.abs(d).T @ np.abs(x)) + FLUSH).all()
+        assert (np.abs(db - d.sum(0)) <= 2 * (M + 2) * U32 * np.abs(d).sum(0)).all()

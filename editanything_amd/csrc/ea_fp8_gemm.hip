@@ -765,9 +765,10 @@ __global__ __launch_bounds__(64) void ea_fp8_wgrad_join_kernel(const float* part
 
 // Kernel (256, 128: the DMA kernels; 0: the one for any N and alignment) and number of slices of the rows: the least time by a model of
 // what was measured.  A 64-row step takes a 256 x 256 workgroup 1.65 us, a 128 x 128 one 0.87 us alone on its CU and 1.25 us beside
-// another; a workgroup's start and end 10 / 5 us; joining s slices 4 us and 2 s + 1 passes over the output at 8 TB/s.
+// another, the any-N kernel's 2.7 and 3.5; a workgroup's start and end 10 / 5 us; joining s slices 4 us and 2 s + 1 passes over the output at 8 TB/s.
 //   16384 x 1280 x 5120 (M x N x K): 256 with 5 slices 216 us (2: 225, 1: 400; 128: 263 at best), 32768 x 2560 x 320: 256 with 12 slices 89
 //   (128 with 8: 103), 8192 x 640 x 640: 128 with 10 slices 25 (1: 111; 256 with 24: 32), 616 x 1280 x 1024: 128 with 1 slice 14 (2: 19; 256: 27)
+//   any N: 616 x 1281 x 1024 5 slices 25.5 (1: 30.3, 2: 25.6), 16384 x 1281 x 1280 9 slices 198 (4: 246, 16: 188), 8192 x 641 x 640 16 slices 46 (8: 63)
 // Workspace and launch go by the same answer, which depends on the sizes alone.
 struct WgradPlan { int kernel, splits, rows; };
 WgradPlan wgrad_plan(int M, int N, int K) {
@@ -787,6 +788,7 @@ WgradPlan wgrad_plan(int M, int N, int K) {
   for (int kernel = 256; kernel >= 0; kernel -= 128) {
     if (kernel ? !dma || (kernel == 256 ? !large || v == 102 : large && v == 101) : dma) continue;
     const int tile = kernel == 256 ? 256 : 128;
+    const double beside = kernel ? 1.25 : 3.5, alone = kernel ? 0.87 : 2.7;      // us per step of a 128 x 128 workgroup
     const long long tiles = (long long)((N + tile - 1) / tile) * ((K + tile - 1) / tile);
     for (int s = 1; s <= steps && s <= 64; ++s) {
       const int per = (steps + s - 1) / s;
@@ -794,7 +796,7 @@ WgradPlan wgrad_plan(int M, int N, int K) {
       if (f && s != f) continue;
       const long long wgs = tiles * s;
       const double t = (kernel == 256 ? (wgs + 255) / 256 * (per * 1.65 + 10)
-                                      : wgs / 512 * (per * 1.25 + 5) + (wgs % 512 > 256 ? per * 1.25 + 5 : wgs % 512 ? per * 0.87 + 5 : 0)) +
+                                      : wgs / 512 * (per * beside + 5) + (wgs % 512 > 256 ? per * beside + 5 : wgs % 512 ? per * alone + 5 : 0)) +
                        (s > 1 ? 4 + (2 * s + 1) * nk * 4 / 8e6 : 0);
       if (w.kernel < 0 || t < best) {
         best = t;

@@ -470,11 +470,12 @@ int ln_bwd_grid(int M, int C) {
 }
 
 // One launch (ea_ln_bwd_few_kernel)?  us, one launch / two: 1 x 1280 2.5 / 6.7, 512 x 1280 3.7 / 8.5, 616 x 1024 in 8 bits 4.2 / 8.5, 1024 x 1280
-// 5.5 / 8.7, 1024 x 4096 10.9 / 19.8, 2048 x 1280 12.6 / 12.1, 4096 x 1280 24.6 / 13.9; the width decides little.  (Rows that start anywhere: 512 x
-// 777 7.4 / 9.8, 1024 x 777 13.1 / 10.1, where the second launch's 3.4 us on the host make up for it.)
-bool ln_bwd_few(int M) {
+// 5.5 / 8.7, 1024 x 4096 10.9 / 19.8, 2048 x 1280 12.6 / 12.1, 4096 x 1280 24.6 / 13.9; the width decides little.  Widths that are not whole vectors
+// cost the walk over all rows more: 512 x 777 7.7 / 10.6, 768 x 777 10.4 / 11.5, 768 x 77 11.1 / 10.6, 768 x 3001 18.3 / 24.1, 1024 x 777
+// 13.6 / 10.8.
+bool ln_bwd_few(int M, int C) {
   const int v = ea_forced_variant();       // tests: 101 pins the one launch, 102 the two
-  return v == 101 || (v != 102 && M <= 1024);
+  return v == 101 || (v != 102 && M <= ((C & 7) ? 768 : 1024));
 }
 
 template <int XK, bool F32, bool ANY>
@@ -523,7 +524,7 @@ extern "C" int ea_layernorm_train(const void* x, int in_f32, const float* gamma,
 }
 
 extern "C" size_t ea_layernorm_bwd_workspace_bytes(int M, int C) {
-  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096 || ln_bwd_few(M)) return 0;
+  if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096 || ln_bwd_few(M, C)) return 0;
   return (size_t)ln_bwd_grid(M, C) * 2 * C * sizeof(float);
 }
 
@@ -534,7 +535,7 @@ extern "C" int ea_layernorm_bwd(const void* dy, const void* x, int x_kind, const
   if (x_kind < XK_F16 || x_kind > XK_FP8) return EA_ERR_BAD_ARG;
   if (M <= 0 || M > EA_FP8_ROWS || C <= 0 || C > 4096) return EA_ERR_BAD_SHAPE;
   if (((uintptr_t)stats & 7) || ((uintptr_t)workspace & 3)) return EA_ERR_BAD_ARG;
-  const bool few = ln_bwd_few(M);
+  const bool few = ln_bwd_few(M, C);
   if (few && !ea_launch_holds(ln_row_groups(M, C) + (C + LF_COLS - 1) / LF_COLS, 256)) return EA_ERR_BAD_SHAPE;
   if (!few && (!workspace || ws_bytes < ea_layernorm_bwd_workspace_bytes(M, C))) return EA_ERR_WORKSPACE;
   const long long es = x_kind == XK_F32 ? 4 : 2, n = (long long)M * C;

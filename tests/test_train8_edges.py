@@ -417,6 +417,18 @@ def test_training_operators_inside_an_autograd_function():
 
 
 # ------------------------------------------------------------------------------------------------------------- launch rules
+def test_launch_rules_follow_the_measurements(emu_lib):
+    """One launch or two of LayerNorm's backward pass, slices of the weight gradient: read off the workspaces."""
+    ln = emu_lib.ea_layernorm_bwd_workspace_bytes
+    for C in (8, 320, 1280, 4096):
+        assert ln(1024, C) == 0 < ln(1025, C)
+    for C in (77, 777, 3001):
+        assert ln(768, C) == 0 < ln(769, C)                    # (1024 x 777: 13.6 us in one launch, 10.8 in two)
+    slices = lambda M, N, K: max(1, emu_lib.ea_gemm_fp8_wgrad_workspace_bytes(M, N, K) // (4 * ((N * K + N + 3) // 4 * 4)))  # noqa: E731
+    assert slices(616, 1280, 1024) == 1 and slices(16384, 1280, 5120) == 5       # the DMA kernels', as before
+    assert slices(616, 1281, 1024) > 1 and slices(16384, 1281, 1280) > 6         # the any-N kernel's steps take three times as long
+
+
 def test_pinned_slices_that_would_leave_one_empty_are_not_taken(emu_lib):
     M, N, K = 600, 24, 100                                     # ten steps: 6, 7, 8 and 9 slices would leave some empty
     q, e = quantize(rows(46, M, K, np.float32))

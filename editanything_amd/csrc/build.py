@@ -47,14 +47,17 @@ def build_hip(force=False, verbose=True):
     deps = srcs + [h if os.path.isabs(h) else os.path.join(HERE, h) for h in HEADERS] + [os.path.abspath(__file__)]
     if not force and not _newer(LIB, deps):
         return LIB
-    objs = []
-    for s in srcs:
+    objs, jobs = [], []
+    for s in srcs:                         # all at once: the longest decides
         o = s[:-4] + ".o"
         cmd = [_hipcc()] + HIP_FLAGS + ["-c", s, "-o", o]
         if verbose:
             print(" ".join(cmd), flush=True)
-        subprocess.check_call(cmd)
+        jobs.append((cmd, subprocess.Popen(cmd)))
         objs.append(o)
+    failed = [cmd for cmd, job in jobs if job.wait()]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
     cmd = [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
     if verbose:
         print(" ".join(cmd), flush=True)

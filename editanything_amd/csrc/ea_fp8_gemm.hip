@@ -15,9 +15,9 @@ namespace {
 // is an fp16 value for -15 <= f <= 7 (the code's smallest step 2^-9 times 2^-15 is fp16's, 448 * 2^7 is 57344).  U belongs to a block column
 // of 128 and is chosen for up to 2048 rows at a time (WxUnit): from the exponents of those rows, and where it changes, the accumulators are
 // multiplied by the power of two between.  Rows that do not fit one window of 23 octaves are taken in several passes over the same rows, each with
-// the others' factors 0 (a block of zeros has E = 0, so padding rows among tiny ones do that).  Choosing a unit costs 0.6 us per 2048 rows: the
-// scale bytes' extremes are joined over the workgroup before the first factor can be written (616 x 1280 x 1024 13.8 -> 14.4 us, 16384 x 1280 x 5120
-// 218 -> 225).
+// the others' factors 0 (a block of zeros has E = 0, so padding rows among tiny ones do that).  Choosing a unit costs 0.4 us (128 x 128
+// tiles) to 1 us per 2048 rows: the scale bytes' extremes are joined over the workgroup before the first factor can be written (616 x 1280 x 1024 13.8 ->
+// 14.2 us, 8192^3 971 -> 988).
 // Both operands have the contracted axis as their ROW axis, so they go to LDS row-major and the fragments are read transposed: 16 lanes
 // take a 4 x 16 (fp16) or 8 x 16 (codes) block and each ends up with consecutive rows of one column.  Bound by the matrix unit at
 // the fp16 rate: 8192^3 905 us = 1215 TFLOP/s (the library's fp16 product: 1382).
@@ -80,6 +80,17 @@ struct WxUnit {
     return away;
   }
 };
+// The lane's number, made anew: what is needed once in 32 steps is not kept in registers over them (kept ones were spilled, and reading a spilled one
+// back waits for all DMA in flight)
+__device__ __forceinline__ int wg_fresh_lane() {
+#ifdef EA_EMU
+  return ea_emu::lane_id();
+#else
+  unsigned z = 0;
+  asm volatile("" : "+s"(z));
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, z));
+#endif
+}
 // Extremes of the bytes of some rows: (hi, 255 - lo) in the halves of a word, whose maximum is taken for both at once
 __device__ __forceinline__ unsigned wx_max(unsigned a, unsigned b) {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -87,9 +98,9 @@ __device__ __forceinline__ unsigned wx_max(unsigned a, unsigned b) {
 }
 __device__ __forceinline__ unsigned wx_word(int byte) { return (unsigned)byte | (unsigned)(255 - byte) << 16; }
 // each wave's word to red[wave]; after a barrier the words of waves first, first + step, ... are joined
-__device__ __forceinline__ void wx_range_put(unsigned* red, unsigned w) {
+__device__ __forceinline__ void wx_range_put(unsigned* red, unsigned w, int lane, int wave) {
   w = ea_f2u(ea_group_reduce<64>(ea_u2f(w), [](float a, float b) { return ea_u2f(wx_max(ea_f2u(a), ea_f2u(b))); }));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = w;
+  if (lane == 0) red[wave] = w;
 }
 template <int FIRST, int STEP, int WAVES>
 __device__ __forceinline__ void wx_range_get(const unsigned* red, WxUnit& x) {
@@ -241,7 +252,7 @@ __global__ __launch_bounds__(256) void ea_fp8_wgrad_kernel(WgradParams p) {
         const int m = c0 + u * 256 + tid;
         w = wx_max(w, wx_word(p.sx[(long long)tk * p.Rp + (m < c1 ? m : c0)]));      // (the first row once more changes nothing)
       }
-      wx_range_put(red, w);
+      wx_range_put(red, w, lane, wave);
       __syncthreads();
       wx_range_get<0, 1, 4>(red, unit);
     }
@@ -487,7 +498,7 @@ __global__ __launch_bounds__(256, 2) void ea_fp8_wgrad_ring_kernel(WgradParams p
         unsigned w = 0;
 #pragma unroll
         for (int u = 0; u < WR_CH * 64 / 256; ++u) w = wx_max(w, wx_word(sb[u]));
-        wx_range_put(red, w);
+        wx_range_put(red, w, lane, wave);
         ea_raw_barrier();
         wx_range_get<0, 1, 4>(red, unit);
       }
@@ -690,7 +701,8 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
   const ea_rows out = ea_make_rows(dw + (long long)n0 * p.K, (long long)(p.N - n0) * p.K * 4);
   bool stored = false;
   auto put = [&](int u) {
-    wg_put(out, acc, [&](int i) { return wm * 128 + (i >> 2) * 64 + ((i & 3) ^ wn) * 16; }, l15, k0 + wn * 64 + 4 * lq, p.K, u, stored);
+    const int fl = wg_fresh_lane();
+    wg_put(out, acc, [&](int i) { return wm * 128 + (i >> 2) * 64 + ((i & 3) ^ wn) * 16; }, fl & 15, k0 + wn * 64 + 4 * (fl >> 4), p.K, u, stored);
     stored = true;
   };
   for (;;) {
@@ -698,11 +710,12 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
     const int n = steps - t0 < WL_CH ? steps - t0 : WL_CH;
     const long long mc = m_begin + t0 * 64ll;
     if (t0 || again) ea_raw_barrier();     // the chunk (pass) before this one has been read
+    const int fl = wg_fresh_lane(), ft = wave * 64 + fl;
     int sb[WL_CH * 128 / 512];
     if (!end) {
-      int kb = 2 * tk + ((tid >> 6) & 1);
+      int kb = 2 * tk + (wave & 1);
       if (kb >= (p.Kp >> 7)) kb = (p.Kp >> 7) - 1;
-      const int mt = (tid >> 7) * 64 + (tid & 63), left = (int)(m_end - mc);
+      const int mt = (wave >> 1) * 64 + fl, left = (int)(m_end - mc);
       const uint8_t* const sx = p.sx + kb * p.Rp + mc;
 #pragma unroll
       for (int u = 0; u < WL_CH * 128 / 512; ++u) sb[u] = sx[mt + u * 256 < left ? mt + u * 256 : left - 1];      // (behind the end: zeros, any factor)
@@ -717,7 +730,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
         unsigned w = 0;
 #pragma unroll
         for (int u = 0; u < WL_CH * 128 / 512; ++u) w = wx_max(w, wx_word(sb[u]));
-        wx_range_put(red, w);                // (even waves: the first block column, odd ones the second)
+        wx_range_put(red, w, fl, wave);      // (even waves: the first block column, odd ones the second)
         ea_raw_barrier();
         wx_range_get<0, 2, 8>(red, unit0);
         wx_range_get<1, 2, 8>(red, unit1);
@@ -732,7 +745,7 @@ __global__ __launch_bounds__(512, 2) void ea_fp8_wgrad_large_kernel(WgradParams 
     wx_rescale(acc, away, old - (wn >> 1 ? unit1.u : unit0.u));
     const int fu = wave & 1 ? unit1.u : unit0.u, from = wave & 1 ? from1 : from0, to = wave & 1 ? to1 : to0;
 #pragma unroll
-    for (int u = 0; u < WL_CH * 128 / 512; ++u) *reinterpret_cast<f16*>(scl + (u * 512 + tid) * 2) = wl_factor(sb[u], fu, from, to);
+    for (int u = 0; u < WL_CH * 128 / 512; ++u) *reinterpret_cast<f16*>(scl + (u * 512 + ft) * 2) = wl_factor(sb[u], fu, from, to);
     ea_wait_dma<2>();
     ea_raw_barrier();
     read_x(0, c0, fb0);

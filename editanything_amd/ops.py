@@ -1046,18 +1046,20 @@ def _refuse(rule, **given):
 
 def _on_device(dev, *tensors):
     """All operands dense and on one MI355X, and none that a recorded graph would have to know of."""
-    if torch.is_grad_enabled():
+    grad = torch.is_grad_enabled()
+    if dev.type == "cuda":
         for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("the 8-bit training operators record no autograd graph, and an operand requires grad: call them under torch.no_grad() or from "
-                                   "an autograd.Function, and their backward operators from its backward pass")
-    if dev.type != "cuda":
-        raise RuntimeError(f"editanything_amd ops run on the MI355X only (an operand is on {dev})")
-    for t in tensors:
-        if t is not None and (t.device != dev or not t.is_contiguous()):
-            if not t.is_cuda:
-                raise RuntimeError(f"editanything_amd ops run on the MI355X only (an operand is on {t.device})")
-            raise ValueError(f"operands must be contiguous and on one device ({dev}): {str(t.dtype)[6:]} {tuple(t.shape)} on {t.device}, strides {tuple(t.stride())}")
+            if t is not None and (t.device != dev or not t.is_contiguous() or (grad and t.requires_grad)):
+                break
+        else:
+            return
+    if grad and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the 8-bit training operators record no autograd graph, and an operand requires grad: call them under torch.no_grad() or from "
+                           "an autograd.Function, and their backward operators from its backward pass")
+    for d in [dev] + [t.device for t in tensors if t is not None]:
+        if d.type != "cuda":
+            raise RuntimeError(f"editanything_amd ops run on the MI355X only (an operand is on {d})")
+    raise ValueError(f"operands must be contiguous and on one device ({dev}): {str(t.dtype)[6:]} {tuple(t.shape)} on {t.device}, strides {tuple(t.stride())}")
 
 
 def _run(dev, what, fn, *args):

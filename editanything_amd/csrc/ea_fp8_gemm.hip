@@ -20,7 +20,7 @@ namespace {
 // 14.2 us, 8192^3 971 -> 988).
 // Both operands have the contracted axis as their ROW axis, so they go to LDS row-major and the fragments are read transposed: 16 lanes
 // take a 4 x 16 (fp16) or 8 x 16 (codes) block and each ends up with consecutive rows of one column.  Bound by the matrix unit at
-// the fp16 rate: 8192^3 905 us = 1215 TFLOP/s (the library's fp16 product: 1382).
+// the fp16 rate: 8192^3 937 us = 1173 TFLOP/s (the library's fp16 product on the same card: 1314).
 // First the kernel for any N and alignment: 128 x 128 tiles, both operands through registers, x decoded on the way to LDS.
 struct WgradParams {
   const f16* dy; const uint8_t* x; const uint8_t* sx;

@@ -15,7 +15,7 @@
 // workgroup in LDS once, written as one partial per workgroup and joined by a second launch in a fixed order: no atomics, so a
 // run repeats bit for bit.  Up to 1024 rows one launch does all of it (ea_ln_bwd_few_kernel).
 // Measured (backward with residual): 16384 x 1280 fp32 52 us = 5.7 TB/s, 32768 x 1280 fp16 without residual 45 us = 5.6 TB/s, 32768 x 320
-// fp16 23 us = 3.7 TB/s, 512 x 1280 3.7 us.  Forward: 32768 x 1280 fp16 30 us = 5.6 TB/s, into 8 bits 28 us.  The next row is in flight
+// fp16 23 us = 3.7 TB/s, 512 x 1280 4.1 us.  Forward: 32768 x 1280 fp16 30 us = 5.6 TB/s, into 8 bits 28 us.  The next row is in flight
 // while one is worked off (without: 16384 x 1280 64 us).
 #include "ea_fp8.h"
 #include "../../include/editanything_hip.h"

@@ -145,7 +145,7 @@ typedef struct ea_tuning {
                                   weights that come from HBM; 101 ... 104: ea_gemm_fp8's 256 x 256, 128 x 128, 64 x 128 and
                                   64 x 64 tiles (102 ... 104 also ea_gemm_fp8_exact's), 101 ... 103: ea_gemm_fp8_wgrad's 256-, 128-column and any-N kernels, 101 / 102:
                                   ea_layernorm_bwd in one / two launches; the rest: tools builds) */
-  int32_t splits;              /* 0 plan's own, s: force the split-K factor */
+  int32_t splits;              /* 0 plan's own, s: force the split-K factor (ea_gemm_fp8_wgrad: the slices of the rows, where that leaves none empty) */
   int32_t bn;                  /* 0 plan's own, 128: force 128-wide column tiles */
   int32_t no_register_direct;  /* 1: LDS-slab epilogue where the register-direct one would run */
   int32_t debug;               /* K-loop / epilogue ablation selector */

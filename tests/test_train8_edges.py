@@ -1,7 +1,6 @@
 """The 8-bit training operators at the edges of their ranges: exponents far from 0 in the weight gradient, and what the entries refuse.
 Plain evaluations in 64 bits and tolerances as in test_train8.py."""
 import ctypes
-import math
 
 import numpy as np
 import pytest
@@ -10,8 +9,8 @@ import torch
 from editanything_amd import _lib as L
 from editanything_amd import ops
 from emu_util import epilogue, ptr
-from test_train8 import (ACT_ABS, GEGLU, GELU, KERNELS, SILU, TINY16, U16, U32, UNIT, act64, decode, encode, force, gemm_case, pack_scales, quantize,
-                         quantize_weight, rows, values)
+from test_train8 import (ACT_ABS, GEGLU, GELU, KERNELS, SILU, TINY16, U16, U32, UNIT, act64, encode, force, gemm_case, pack_scales, quantize, rows,
+                         values)
 
 FLUSH = 2.0 ** -126                        # fp32's smallest normal number: what lies below may be flushed
 
